@@ -211,10 +211,11 @@ def _compile(state):
     def zeros(shape, dtype):
         return cgt.shared(np.zeros(shape, dtype), fixed_shape_mask="all")
 
-    case, x = state["case"], shared(state["x"])
+    case = state["case"]
     kind, rows, cols = case["kind"], case["rows"], case["cols"]
     float_type, more = case.get("dtype", "f4"), []
     with cgt.scoped_update_config(precision="double" if float_type == "f8" else "single"):
+        x = shared(state["x"])
         if kind in ("norm", "norm_train"):
             gain, bias = shared(state["gain"]), shared(state["bias"])
             y = nn.layer_norm(x, gain, bias, epsilon=EPSILON)
