@@ -2458,7 +2458,7 @@ def determine_devices(nodes_sorted, updatetarg2src):
         if node.is_scalar():
             device = home_device
         elif node in updatetarg2src:
-            device = node2dev[updatetarg2src[node]]
+            device = updatetarg2src[node].op.device
             assert "native_" + device.devtype in node.op.available_impls, \
                 "update only works if final operation can be performed on target device"
         elif node.is_data():
@@ -2751,7 +2751,7 @@ def determine_memowner(nodes_sorted, updates, node2dev, outputs, node2shape, con
             for parent in node.parents:
                 parentowner = node2memowner[parent]
                 if (len(node2child[parent]) == 1 and node.dtype == parent.dtype and is_tensor(parent)
-                        and node2dev[node] == node2dev[parent]
+                        and node in node2dev and node2dev[node] == node2dev.get(parent)   # not an extent's arithmetic: allocations read it
                         and _is_data_mutable(parentowner) and parentowner is parent
                         and parent not in outputs and parent not in const_nodes
                         and _same_shape(node2shape[node], node2shape[parent])):
@@ -2844,6 +2844,52 @@ def create_execution_graph(inputs, nodes_sorted, node2shape, node2memowner, node
     return ExecutionGraph(instrs, len(inputs), counter.count), node2memloc
 
 
+def _memory_held(instrs):
+    """location -> the locations whose memory it may be: its own, or those that it views"""
+    holds = {}
+    for ins in instrs:
+        held = holds.setdefault(ins.write_loc.index, {ins.write_loc.index})
+        if isinstance(ins, (ReturnByVal, BuildTup)):
+            held.update(*[holds[r.index] for r in ins.read_locs if r.index in holds])
+    return holds
+
+
+def place_results_in_variables(eg, variable_types):
+    """Instruction-list pass: a variable whose new value is one of several results of an operation (the gradient of a layer
+    norm's input, kept by the caller) is written by the operation itself instead of being copied into. `variable_types`:
+    location index -> type of the variables. Only where no instruction from the operation up to the copy touches the
+    variable's memory, the operation's operands among them: every reader still sees the value it saw before."""
+    instrs = eg.instrs
+    holds = _memory_held(instrs)
+
+    def touches(ins, loc):
+        return any(loc in holds[r.index] for r in getattr(ins, "read_locs", [])) or loc in holds[ins.write_loc.index]
+    writer, built, defined, part = {}, {}, {}, {}    # by location; part: a result's location -> (tuple's location, place)
+    drop, placed = set(), set()
+    for (i, ins) in enumerate(instrs):
+        w = ins.write_loc.index
+        defined.setdefault(w, i)
+        if isinstance(ins, BuildTup):
+            built[w] = i
+        elif isinstance(ins, ReturnByRef) and w in built and ins.op.results_in_variables and not ins.once:
+            writer[w] = i
+        elif isinstance(ins, ReturnByVal) and isinstance(ins.op, core.TupleIndex) and ins.read_locs[0].index in writer:
+            part[w] = (ins.read_locs[0].index, ins.op.idx)
+        elif (isinstance(ins, ReturnByRef) and isinstance(ins.op, core.ElwiseUnary) and ins.op.opname.startswith("cast_to_")
+              and w in variable_types and ins.read_locs[0].index in part):
+            (tup, k) = part[ins.read_locs[0].index]
+            build = instrs[built[tup]]
+            if (tup, k) in placed or build.typ[k] != variable_types[w] or build.read_locs[k].devtype != ins.write_loc.devtype:
+                continue
+            if defined[w] > built[tup] or any(touches(instrs[j], w) for j in range(writer[tup], i)):
+                continue
+            own = build.read_locs[k].index
+            drop.update([i] + [j for (j, other) in enumerate(instrs) if isinstance(other, Alloc) and other.write_loc.index == own])
+            build.read_locs[k] = ins.write_loc
+            placed.add((tup, k))
+    eg.instrs = [ins for (i, ins) in enumerate(instrs) if i not in drop]
+
+
 def merge_parameter_updates(eg, update_locs):
     """Instruction-list pass: the update instructions of a step that run one and the same single-output FusedElwise
     program on float32 tensors / scalars (SGD: p - lr * g for every parameter) become ONE MultiFusedElwise instruction
@@ -2852,11 +2898,7 @@ def merge_parameter_updates(eg, update_locs):
     memory of its result, nor writes memory that it reads, itself or through a view: every reader still sees the value it
     saw before. Two updates of one launch run side by side, so neither may read what the other writes."""
     instrs = eg.instrs
-    holds = {}    # location -> the locations whose memory it may be: its own, or those that it views
-    for ins in instrs:
-        held = holds.setdefault(ins.write_loc.index, {ins.write_loc.index})
-        if isinstance(ins, (ReturnByVal, BuildTup)):
-            held.update(*[holds[r.index] for r in ins.read_locs if r.index in holds])
+    holds = _memory_held(instrs)
 
     def memory(locs):
         return set().union(*[holds[loc.index] for loc in locs])
@@ -2991,21 +3033,27 @@ def execution_graph(inputs, outputs, updates, givens):
     all_out = outputs_simple + updatetargs_simple
 
     nodelist = core.topsorted(all_out)
+    read = set(nodelist)
+    unread = [v for v in updatesrcs if v not in read]    # variables that are only written
+    nodelist = unread + nodelist
     node2dev = determine_devices(nodelist, dict(zip(updatetargs_simple, updatesrcs)))
     add_transports(nodelist, node2dev, node2shape)
 
     updates_simple = list(zip(updatesrcs, updatetargs_simple))
     keep_old_values(all_out, updates_simple, node2dev, node2shape)
     extra = _update_control_deps(all_out, updates_simple)
+    for (v, target) in updates_simple:     # the memory that the target is computed in
+        extra[target] = extra.get(target, []) + [v]
     first, last = _transport_schedule(all_out, updatetargs_simple, node2dev)
     for node in last:
         extra[node] = extra.get(node, []) + [t for t in updatetargs_simple if t is not node]
-    nodes_sorted = topsorted_shapes_first(first + all_out, node2shape, extra)
+    nodes_sorted = topsorted_shapes_first(first + unread + all_out, node2shape, extra)
     const_nodes = compute_const_nodes(nodes_sorted)
     node2memowner = determine_memowner(nodes_sorted, updates_simple, node2dev, outputs_simple, node2shape, const_nodes)
     written_into = set(owner for (n, owner) in node2memowner.items() if owner is not n)
     once_nodes = set(n for n in const_nodes if n not in written_into)
     eg, node2memloc = create_execution_graph(inputs, nodes_sorted, node2shape, node2memowner, node2dev, once_nodes)
+    place_results_in_variables(eg, {node2memloc[v].index: v.typ for v in updatesrcs})
     if config["merge_parameter_updates"] and updates_simple:
         merge_parameter_updates(eg, set(node2memloc[t].index for t in updatetargs_simple))
     if config["delay_host_arithmetic"]:

@@ -375,6 +375,7 @@ class Op(object):
     available_impls = ()
     is_data_op = False
     is_random_op = False
+    results_in_variables = False   # several results: each may be the memory of a variable whose new value it is
 
     def shp_apply(self, parents):
         raise NotImplementedError

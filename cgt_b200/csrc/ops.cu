@@ -690,6 +690,75 @@ OP_BYREF(cgtb_op_lrn_backward) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// Layer norm, dropout, 8-bit rows and their product (no counterparts in the reference)
+// ------------------------------------------------------------------------------------------------
+static long rows_of(cgtArray* x) { long n = 1; for (int i = 0; i + 1 < x->ndim(); ++i) n *= x->shape()[i]; return n; }
+static long cols_of(cgtArray* x) { return x->shape()[x->ndim() - 1]; }
+static bool norm_operands(const char* op, cgtArray* x, std::initializer_list<cgtArray*> full, std::initializer_list<cgtArray*> columns) {
+  if (x->ndim() < 1) { fail("%s: takes an array of at least one dimension", op); return false; }
+  for (auto a : full)
+    if (!on_gpu(a) || a->dtype() != x->dtype() || a->size() != x->size()) { fail("%s: operands do not fit together", op); return false; }
+  for (auto a : columns)
+    if (!on_gpu(a) || a->dtype() != x->dtype() || a->size() != cols_of(x)) {
+      fail("%s: gain and bias need one value for each of the %ld columns", op, cols_of(x));
+      return false;
+    }
+  return true;
+}
+struct NormClosure { double epsilon; };
+OP_BYREF(cgtb_op_layer_norm_forward) {  // x, gain, bias -> y
+  cgtArray *x = ARR(reads[0]), *gain = ARR(reads[1]), *bias = ARR(reads[2]), *y = ARR(write0);
+  if (!norm_operands("LayerNorm", x, {x, y}, {gain, bias})) return;
+  cgtb_layer_norm_forward(x->dtype(), x->data(), rows_of(x), cols_of(x), gain->data(), bias->data(), ((NormClosure*)cl0)->epsilon, y->data());
+}
+OP_BYREF(cgtb_op_layer_norm_backward) {  // x, gain, gy -> (dx, dgain, dbias)
+  cgtTuple* out = (cgtTuple*)write0;
+  cgtArray *x = ARR(reads[0]), *gain = ARR(reads[1]), *gy = ARR(reads[2]);
+  cgtArray *dx = ARR(out->getitem(0)), *dgain = ARR(out->getitem(1)), *dbias = ARR(out->getitem(2));
+  if (!norm_operands("LayerNormBackward", x, {x, gy, dx}, {gain, dgain, dbias})) return;
+  cgtb_layer_norm_backward(x->dtype(), x->data(), gain->data(), gy->data(), rows_of(x), cols_of(x), ((NormClosure*)cl0)->epsilon, dx->data(),
+                           dgain->data(), dbias->data());
+}
+struct DropoutClosure { double p; int site; };
+OP_BYREF(cgtb_op_dropout) {  // x, state -> y
+  DropoutClosure* cl = (DropoutClosure*)cl0;
+  cgtArray *x = ARR(reads[0]), *state = ARR(reads[1]), *y = ARR(write0);
+  if (!all_gpu({x, state, y}) || y->dtype() != x->dtype() || y->size() != x->size() || state->dtype() != cgt_i8 || state->size() != 2) {
+    fail("Dropout: operands do not fit together");
+    return;
+  }
+  cgtb_dropout(x->dtype(), x->data(), x->size(), cl->p, (const int64_t*)state->data(), (unsigned)cl->site, y->data());
+}
+OP_BYREF(cgtb_op_quantize_rows) {  // x -> (codes, scales)
+  cgtTuple* out = (cgtTuple*)write0;
+  cgtArray *x = ARR(reads[0]), *codes = ARR(out->getitem(0)), *scales = ARR(out->getitem(1));
+  if (!all_gpu({x, codes, scales}) || x->dtype() != cgt_f4 || x->ndim() != 2 || codes->size() != x->shape()[0] * (cgtb_ceil_div(x->shape()[1], 16) * 16)) {
+    fail("QuantizeRows: takes a float32 matrix on the GPU");
+    return;
+  }
+  cgtb_quantize_rows((const float*)x->data(), x->shape()[0], x->shape()[1], (int8_t*)codes->data(), (float*)scales->data());
+}
+struct Int8ProductClosure { int has_bias; };
+OP_BYREF(cgtb_op_int8_product) {  // codes, scales, weight codes, weight scales (, bias) -> y
+  const bool has_bias = ((Int8ProductClosure*)cl0)->has_bias != 0;
+  cgtArray *a = ARR(reads[0]), *sa = ARR(reads[1]), *b = ARR(reads[2]), *sb = ARR(reads[3]), *y = ARR(write0);
+  cgtArray* bias = has_bias ? ARR(reads[4]) : nullptr;
+  if (!all_gpu({a, sa, b, sb, y}) || (bias && !on_gpu(bias))) { fail("Int8Product: operands must be on the GPU"); return; }
+  if (a->dtype() != cgt_i1 || b->dtype() != cgt_i1 || a->ndim() != 2 || b->ndim() != 2 || a->shape()[1] != b->shape()[1]) {
+    fail("Int8Product: needs two matrices of codes with rows of one length");
+    return;
+  }
+  const long M = a->shape()[0], N = b->shape()[0];
+  if (sa->size() != M || sb->size() != N || (bias && bias->size() != N) || y->size() != M * N || sa->dtype() != cgt_f4 || sb->dtype() != cgt_f4 ||
+      (bias && bias->dtype() != cgt_f4)) {
+    fail("Int8Product: needs a float32 scale for each of the %ld rows and each of the %ld output channels", M, N);
+    return;
+  }
+  cgtb_int8_product((const int8_t*)a->data(), (const float*)sa->data(), (const int8_t*)b->data(), (const float*)sb->data(),
+                    bias ? (const float*)bias->data() : nullptr, M, N, a->shape()[1], (float*)y->data());
+}
+
+// ------------------------------------------------------------------------------------------------
 // Sum / Max (cgt/core.py:1687-1738). axes are a bit mask.
 // ------------------------------------------------------------------------------------------------
 struct ReduceClosure { int kind; int axes_mask; };

@@ -10,6 +10,9 @@ import numpy as np
 from . import core
 from .nn_ops.im2col import im2col
 from .nn_ops.cross_channel_lrn import cross_channel_lrn  # noqa: F401  (re-exported)
+from .nn_ops.dropout import RandomStream, dropout  # noqa: F401  (re-exported)
+from .nn_ops.int8 import Int8Affine, int8_product, quantize_rows  # noqa: F401  (re-exported)
+from .nn_ops.layer_norm import layer_norm
 from .nn_ops.max_pool_2d import MaxPool, PoolInfo
 
 
@@ -157,6 +160,19 @@ class Affine(object):
 
     def __call__(self, x):
         return _cgt().broadcast("+", x.dot(self.weight), self.bias, "xx,1x")
+
+
+class LayerNorm(object):
+    """layer_norm over rows of `size` values, with gain (from 1) and bias (from 0) as parameters."""
+
+    def __init__(self, size, name=None, epsilon=1e-5):
+        name = "unnamed" if name is None else name
+        self.epsilon = epsilon
+        self.gain = parameter(init_array(Constant(1), (int(size),)), name=name + ".gain")
+        self.bias = parameter(init_array(Constant(0), (int(size),)), name=name + ".bias")
+
+    def __call__(self, x):
+        return layer_norm(x, self.gain, self.bias, self.epsilon)
 
 
 class SpatialConvolution(object):

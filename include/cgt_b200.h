@@ -193,6 +193,35 @@ int cgtb_lrn_forward(int dtype, const void* x, long N, int C, int H, int W, int 
 int cgtb_lrn_backward(int dtype, const void* x, const void* top, const void* scale, const void* gtop, long N, int C,
                       int H, int W, int size, double alpha, double beta, void* gx);
 
+/* Layer norm over the rows of an [R, C] matrix (no counterpart in the reference, whose only norm is the LRN above):
+ *   y[r, c] = (x[r, c] - m) / sqrt(v + epsilon) * gain[c] + bias[c], m and v the mean and variance of row r.
+ * Backward, with xh = (x - m) / sqrt(v + epsilon) and d = gy * gain:
+ *   dx = (d - mean(d) - xh * mean(d * xh)) / sqrt(v + epsilon), dgain[c] = sum_r gy * xh, dbias[c] = sum_r gy.
+ * The backward pass takes x and not y or saved statistics: it reads x anyway and forms them again. float32 and float64,
+ * sums in the arrays' type, always in the same order. Any R and C >= 0; results may not overlap operands. */
+int cgtb_layer_norm_forward(int dtype, const void* x, long R, long C, const void* gain, const void* bias, double epsilon, void* y);
+int cgtb_layer_norm_backward(int dtype, const void* x, const void* gain, const void* gy, long R, long C, double epsilon, void* dx,
+                             void* dgain, void* dbias);
+
+/* Dropout of n values, float32 or float64: y[i] = x[i] / (1 - p), or 0 where the element is dropped, whatever x[i] is. No mask
+ * is stored: element i is dropped where word i % 4 of the Philox4x32-10 block with key (seed, seed >> 32) and counter
+ * (i / 4, i / 4 >> 32, step, site) is below round(p * 2^32). state: two int64 in device memory, seed and step, read by the
+ * kernel, so that a captured graph drops other elements when its step has changed; the masks repeat after 2^32 steps. The
+ * gradient is the same call on the gradient of y. 0 <= p < 1; y may be x. */
+int cgtb_dropout(int dtype, const void* x, long n, double p, const int64_t* state, unsigned site, void* y);
+
+/* Rows in 8-bit integers, x [R, C] float32: scales[r] = max_c |x[r, c]| / 127, codes[r, c] = 127 x[r, c] / max |x[r, :]| rounded
+ * to the nearest whole number, ties to the even one, exactly. Rows of codes are C rounded up to a multiple of 16 long, the
+ * rest zeros. A row of zeros: scale and codes 0; a row that holds an infinity or a NaN: scale NaN, codes 0. */
+int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, float* scales);
+/* y[m, n] = (sum_k a[m, k] * b[n, k]) * sa[m] * sb[n] + bias[n]: a product of 8-bit integers with a scale for each row of a (a
+ * token) and each row of b (an output channel). a [M, K], b [N, K] int8 as cgtb_quantize_rows writes them: K a multiple of 16
+ * and below CGTB_INT8_MAX_K, 16-byte aligned; the sum is exact in 32-bit integers, whatever the codes. sa [M], sb [N], bias
+ * [N] or null, y [M, N]: float32. */
+#define CGTB_INT8_MAX_K 131072
+int cgtb_int8_product(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K,
+                      float* y);
+
 /* Data gradient of a stride-1 convolution in one kernel. Replaces the pair Mul22(dy, W) + Col2Im that the
  * reference's graph holds for it (cgt/nn_ops/im2col.py:Im2Col.pullback, include/im2col.h:30-50): no column
  * matrix is written or read.

@@ -1,0 +1,202 @@
+"""Layer norm, dropout, 8-bit rows and 8-bit products without a GPU: the generator's published answers, refusals when a
+graph is built, and which memory a step's results go to."""
+import numpy as np
+import pytest
+
+import cgt_b200 as cgt
+from cgt_b200 import compilation, core, nn
+from cgt_b200.nn_ops import dropout as dropout_ops
+from cgt_b200.nn_ops import int8 as int8_ops
+from cgt_b200.nn_ops import layer_norm as norm_ops
+from tests import block_ops as ref
+from tests.host_run import HostRun
+
+
+def test_the_generator_gives_the_published_answers():
+    """Known answers of Philox4x32-10 from its authors: counter and key all zeros, and all ones."""
+    assert [int(w) for w in ref.philox([0], 0, 0, 0)[0]] == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = 0xFFFFFFFFFFFFFFFF
+    assert [int(w) for w in ref.philox([np.uint64(ones)], ones, 0xFFFFFFFF, ones)[0]] == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+def test_the_share_of_dropped_elements():
+    n = 1 << 18
+    for (p, seed, step, site) in ((0.1, 0, 0, 0), (0.5, 3, 100, 2), (0.85, -1, 7, 5)):
+        # a binomial count is within five of its standard deviations, sqrt(p (1 - p) n), but for one time in a million
+        assert abs((~ref.kept(n, p, seed, step, site)).sum() - p * n) < 5 * np.sqrt(p * (1 - p) * n)
+
+
+def test_host_quantization_is_the_operators():
+    rs = np.random.RandomState(0)
+    x = rs.randn(30, 37).astype("f4")
+    x[3], x[4, 5], x[5, 6], x[6] = 0, np.nan, np.inf, rs.randint(-254, 255, 37) / 2.0
+    x[6, 0] = 127
+    for (a, b) in zip(int8_ops._quantize(x), ref.quantize(x)):
+        assert a.dtype == b.dtype and np.array_equal(a, b, equal_nan=True)
+
+
+def test_refusals():
+    x, v, i = cgt.matrix("x"), cgt.vector("v"), cgt.matrix("i", dtype="i8")
+    stream = nn.RandomStream(0)
+    for build in (lambda: nn.layer_norm(i, v, v), lambda: nn.layer_norm(x, x, v), lambda: nn.layer_norm(x, v, cgt.vector("k", dtype="i8")),
+                  lambda: nn.layer_norm(cgt.scalar("s"), v, v), lambda: nn.layer_norm(x, v, v, epsilon=-1.0), lambda: nn.layer_norm(x, v, v, epsilon=float("nan")),
+                  lambda: nn.layer_norm(x, v, v, epsilon=float("inf")), lambda: nn.dropout(x, 1.0, stream), lambda: nn.dropout(x, -0.1, stream),
+                  lambda: nn.dropout(x, float("nan"), stream), lambda: nn.dropout(x, 0.5, 7), lambda: nn.dropout(i, 0.5, stream),
+                  lambda: nn.dropout(cgt.scalar("s"), 0.5, stream), lambda: nn.quantize_rows(v), lambda: nn.quantize_rows(i),
+                  lambda: nn.int8_product(x, v, x, v), lambda: nn.int8_product(cgt.matrix("c", dtype="i1"), v, cgt.matrix("d", dtype="i1"), x)):
+        with pytest.raises(ValueError):
+            build()
+    with cgt.scoped_update_config(precision="double"):
+        with pytest.raises(ValueError):
+            nn.quantize_rows(cgt.matrix("x"))
+        with pytest.raises(ValueError):
+            nn.Int8Affine(nn.Affine(3, 4))
+    with pytest.raises(ValueError):
+        nn.Int8Affine(nn.Affine(131072, 1))
+    assert nn.dropout(x, 0.0, stream) is x
+
+
+def test_no_gradient_where_there_is_none():
+    x = cgt.shared(np.ones((3, 16), "f4"), fixed_shape_mask="all")
+    codes, scales = nn.quantize_rows(x)
+    with pytest.raises(Exception):
+        cgt.grad(scales.sum(), [x])
+
+
+def test_every_dropout_of_a_stream_has_elements_of_its_own():
+    x = cgt.matrix("x", fixed_shape=(4, 4))
+    stream = nn.RandomStream(0)
+    y = nn.dropout(x, 0.5, stream) + nn.dropout(x, 0.5, stream)
+    eg = compilation.execution_graph([x], [y], [], [])[0]
+    assert sorted(i.op.site for i in eg.instrs if isinstance(getattr(i, "op", None), dropout_ops.Dropout)) == [0, 1]
+
+
+# ------------------------------------------------------------------------------------------------
+# results that are variables: the compiled instruction list, executed on numpy arrays
+# ------------------------------------------------------------------------------------------------
+class _Run(HostRun):
+    def _into(self, ins, reads, write):
+        op = ins.op
+        writes = write if isinstance(write, tuple) else (write,)
+        if isinstance(op, norm_ops.LayerNorm):
+            results = [ref.norm(*reads, op.epsilon)[0]]
+        elif isinstance(op, norm_ops.LayerNormBackward):
+            results = ref.norm_gradients(*reads, op.epsilon)
+        elif isinstance(op, int8_ops.QuantizeRows):
+            results = ref.quantize(reads[0])
+        elif isinstance(op, dropout_ops.Dropout):
+            results = [ref.dropout(reads[0], op.p, int(reads[1][0]), int(reads[1][1]), op.site)]
+        else:
+            return HostRun._into(self, ins, reads, write)
+        for out in writes:
+            assert not any(np.shares_memory(r, out) for r in reads), "%r reads the memory that it overwrites" % (op,)
+        results = [np.array(r, copy=True) for r in results]
+        for (out, r) in zip(writes, results):
+            assert out.shape == r.shape
+            out[...] = r
+
+
+def _var(rs, *shape):
+    return cgt.shared(rs.randn(*shape).astype("f4"), fixed_shape_mask="all")
+
+
+def _copies(run):
+    return sum(isinstance(op, core.ElwiseUnary) and op.opname.startswith("cast_to_") for op in run.ops())
+
+
+def _case():
+    rs = np.random.RandomState(0)
+    x, gain, bias, gy = _var(rs, 6, 20), _var(rs, 20), _var(rs, 20), _var(rs, 6, 20)
+    y = nn.layer_norm(x, gain, bias)
+    old = [v.op.get_value() for v in (x, gain, bias, gy)]
+    wants = [ref.norm(*old[:3], 1e-5)[0]] + list(ref.norm_gradients(old[0], old[1], old[3], 1e-5))
+    return rs, (x, gain, bias, gy), [y] + core.pullback([y], [gy], [x, gain, bias]), [w.astype("f4") for w in wants]
+
+
+def test_several_results_go_into_their_variables():
+    rs, _inputs, news, wants = _case()
+    outs = [_var(rs, *w.shape) for w in wants]
+    run = _Run([], [], list(zip(outs, news)))
+    assert _copies(run) == 0
+    run()
+    assert all(np.array_equal(run.value(o), w) for (o, w) in zip(outs, wants))
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (1, 0, 3, 2), (3, 2, 1, 0)])
+def test_results_that_replace_operands(order):
+    """x, gain, bias and gy get, in some order, the results that are computed from them."""
+    _rs, (x, gain, bias, gy), news, wants = _case()
+    targets = dict(zip(range(4), ((gy, 0), (x, 1), (gain, 2), (bias, 3))))
+    pairs = [targets[k] for k in order]
+    run = _Run([], [], [(v, news[i]) for (v, i) in pairs])
+    run()
+    assert all(np.array_equal(run.value(v), wants[i]) for (v, i) in pairs)
+
+
+def test_a_variable_that_is_still_read_after_the_operation():
+    """A reader of the old value that the order puts behind the operation: the operation may not write the variable."""
+    rs, (x, gain, bias, gy), news, wants = _case()
+    keep = _var(rs, 6, 20)
+    old = keep.op.get_value()
+    later = cgt.tanh(keep * news[1])       # needs dx and the old value
+    out = _var(rs, 6, 20)
+    run = _Run([], [later], [(keep, news[1]), (out, keep + 1.0)])
+    for _ in range(2):
+        got = run()[0]
+        np.testing.assert_allclose(got, np.tanh(old * wants[1]), rtol=1e-6)
+        np.testing.assert_allclose(run.value(out), old + 1, rtol=1e-6)
+        assert np.array_equal(run.value(keep), wants[1])
+        old = wants[1]
+
+
+def test_one_result_for_two_variables_and_for_the_caller():
+    rs, _inputs, news, wants = _case()
+    a, b = _var(rs, 20), _var(rs, 20)
+    run = _Run([], [news[2], news[2] * 2.0], [(a, news[2]), (b, news[2])])
+    got = run()
+    assert np.array_equal(run.value(a), wants[2]) and np.array_equal(run.value(b), wants[2])
+    assert np.array_equal(got[0], wants[2]) and np.array_equal(got[1], 2 * wants[2])
+
+
+def test_a_result_goes_into_no_variable_of_another_type():
+    """scales (float32) into an int64 variable: copied, as before."""
+    x = cgt.shared(np.ones((5, 16), "f4"), fixed_shape_mask="all")
+    v = cgt.shared(np.zeros(5, "i8"), fixed_shape_mask="all")
+    eg = compilation.execution_graph([], [], [(v, nn.quantize_rows(x)[1])], [])[0]
+    assert any(getattr(getattr(i, "op", None), "opname", "").startswith("cast_to_") for i in eg.instrs)
+
+
+def test_variables_that_nothing_reads():
+    """A variable that is only written, from a chain, a product and a copy."""
+    rs = np.random.RandomState(0)
+    a, b = _var(rs, 8, 8), _var(rs, 8, 8)
+    outs = [_var(rs, 8, 8) for _ in range(3)]
+    run = HostRun([], [], [(outs[0], cgt.tanh(a + b)), (outs[1], a.dot(b)), (outs[2], a.reshape([8, 8]))])
+    run()
+    (av, bv) = (a.op.get_value(), b.op.get_value())
+    np.testing.assert_allclose(run.value(outs[0]), np.tanh(av + bv), rtol=1e-5)
+    np.testing.assert_allclose(run.value(outs[1]), av @ bv, rtol=1e-4, atol=1e-5)
+    assert np.array_equal(run.value(outs[2]), av)
+
+
+def test_dropout_in_a_step_on_the_host():
+    rs = np.random.RandomState(0)
+    x = _var(rs, 10, 7)
+    old = x.op.get_value()
+    stream = nn.RandomStream(9)
+    y = nn.dropout(x, 0.3, stream)
+    run = _Run([], [y], [(x, nn.dropout(y, 0.5, stream))] + stream.updates())
+    for step in range(3):
+        got = run()[0]
+        want = ref.dropout(old, 0.3, 9, step, 0)
+        assert np.array_equal(got, want)
+        old = ref.dropout(want, 0.5, 9, step, 1)
+        assert np.array_equal(run.value(x), old)
+
+
+def test_an_extent_that_is_computed_from_an_open_one():
+    x = cgt.matrix("x")
+    run = _Run([x], list(nn.quantize_rows(x)))
+    for shape in ((3, 20), (5, 16), (2, 1)):
+        v = np.random.RandomState(0).randn(*shape).astype("f4")
+        assert all(np.array_equal(a, b) for (a, b) in zip(run(v), ref.quantize(v)))

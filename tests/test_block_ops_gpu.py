@@ -1,0 +1,470 @@
+"""Layer norm, dropout, 8-bit rows and 8-bit products on the GPU against tests/block_ops.py, at the sizes where the kernels
+change their form, and in compiled functions."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import cgt_b200 as cgt
+from cgt_b200 import core, nn, runtime
+from tests import block_ops as ref
+from tests.gpu_util import Dev, call, code
+
+pytestmark = pytest.mark.gpu
+
+ROWS_COLS = [(1, 1), (3, 2), (5, 3), (2, 4), (7, 31), (33, 32), (130, 33), (1, 256), (128, 256), (9, 255), (257, 128), (64, 784), (37, 1000), (5, 1001),
+             (11, 1024), (6, 1028), (300, 2048), (19, 2050), (21, 4096), (8, 4097), (4, 8192), (3, 8200), (5, 12345), (2, 20000), (3000, 4), (5001, 17)]
+
+
+def _norm_inputs(R, C, dtype, seed=0):
+    rs = np.random.RandomState(seed)
+    x = (rs.randn(R, C) * np.exp(rs.randn(R, 1)) + 3 * rs.randn(R, 1)).astype(dtype)
+    return x, (1 + 0.3 * rs.randn(C)).astype(dtype), rs.randn(C).astype(dtype), rs.randn(R, C).astype(dtype)
+
+
+def _forward(x, gain, bias, eps):
+    y = Dev(np.full(x.shape, 7, x.dtype))
+    dx, dg, db = Dev(x), Dev(gain), Dev(bias)
+    call("cgtb_layer_norm_forward", code(x.dtype), dx.ptr, x.shape[0], x.shape[1], dg.ptr, db.ptr, eps, y.ptr)
+    return y.get()
+
+
+def _backward(x, gain, gy, eps):
+    outs = [Dev(np.full(x.shape, 7, x.dtype)), Dev(np.full(gain.shape, 7, x.dtype)), Dev(np.full(gain.shape, 7, x.dtype))]
+    dx, dg, dy = Dev(x), Dev(gain), Dev(gy)
+    call("cgtb_layer_norm_backward", code(x.dtype), dx.ptr, dg.ptr, dy.ptr, x.shape[0], x.shape[1], eps, *[o.ptr for o in outs])
+    return [o.get() for o in outs]
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("R,C", ROWS_COLS)
+def test_layer_norm(rt, R, C, dtype):
+    x, gain, bias, gy = _norm_inputs(R, C, dtype)
+    eps = 1e-5
+    bounds = ref.norm_bounds(x, gain, bias, gy, eps)
+    wants = (ref.norm(x, gain, bias, eps)[0],) + tuple(ref.norm_gradients(x, gain, gy, eps))
+    for (name, got, want, bound) in zip(("y", "dx", "dgain", "dbias"), [_forward(x, gain, bias, eps)] + _backward(x, gain, gy, eps), wants, bounds):
+        off = np.abs(got - want)
+        assert (off <= bound).all(), (name, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("C", [5, 64, 1000, 5000])
+def test_layer_norm_of_rows_far_from_zero(rt, C, dtype):
+    """A common offset of 1000 spreads: the variance is that of the centred values, not a difference of large sums."""
+    rs = np.random.RandomState(1)
+    x = (rs.randn(40, C) + 1000).astype(dtype)
+    gain, bias = np.ones(C, dtype), np.zeros(C, dtype)
+    assert (np.abs(_forward(x, gain, bias, 1e-5) - ref.norm(x, gain, bias, 1e-5)[0]) <= ref.norm_bounds(x, gain, bias, None, 1e-5)).all()
+
+
+@pytest.mark.parametrize("C", [8, 300, 4096, 9000])
+def test_layer_norm_keeps_rows_apart(rt, C):
+    """Rows of equal values, of zeros, and with an infinity or a NaN: only the last two are NaN, in themselves and, as the sum
+    over all rows has to be, in the gradient of the gain."""
+    x, gain, bias, gy = _norm_inputs(12, C, "f4")
+    x[2], x[3] = 0, 5
+    want, bounds = ref.norm(x, gain, bias, 1e-5)[0], ref.norm_bounds(x, gain, bias, gy, 1e-5)
+    dx = ref.norm_gradients(x, gain, gy, 1e-5)[0]
+    bad = x.copy()
+    bad[5, C // 2], bad[7, C - 1] = np.inf, np.nan
+    fine = [r for r in range(12) if r not in (5, 7)]
+    y = _forward(bad, gain, bias, 1e-5)
+    gx, dgain, dbias = _backward(bad, gain, gy, 1e-5)
+    assert np.isnan(y[[5, 7]]).all() and np.isnan(gx[[5, 7]]).all() and np.isnan(dgain).all() and np.isfinite(dbias).all()
+    assert (np.abs(y - want) <= bounds[0])[fine].all() and (np.abs(gx - dx) <= bounds[1])[fine].all()
+
+
+def test_layer_norm_without_rows(rt):
+    x, gain, bias, gy = _norm_inputs(0, 40, "f4")
+    assert _forward(x, gain, bias, 1e-5).shape == (0, 40)
+    assert [np.abs(g).sum() for g in _backward(x, gain, gy, 1e-5)] == [0, 0, 0]
+
+
+@pytest.mark.parametrize("R,C,dtype", [(128, 256, "f4"), (700, 1000, "f8"), (70, 9000, "f4")])
+def test_layer_norm_is_reproducible(rt, R, C, dtype):
+    x, gain, bias, gy = _norm_inputs(R, C, dtype)
+    first = _backward(x, gain, gy, 1e-5)
+    for _ in range(3):
+        assert all(np.array_equal(a, b) for (a, b) in zip(first, _backward(x, gain, gy, 1e-5)))
+
+
+def test_layer_norm_gradients_against_differences(rt):
+    rs = np.random.RandomState(3)
+    x, gain, bias, gy = _norm_inputs(4, 9, "f8")
+    got = _backward(x, gain, gy, 1e-3)
+
+    def loss(x, gain, bias):
+        return float((_forward(x, gain, bias, 1e-3) * gy).sum())
+    h = 1e-5
+    for (k, g) in enumerate(got):
+        for _ in range(6):
+            args = [x.copy(), gain.copy(), bias.copy()]
+            at = tuple(rs.randint(n) for n in args[k].shape)
+            args[k][at] += h
+            up = loss(*args)
+            args[k][at] -= 2 * h
+            # central differences: h^2 times the third derivative (some units here, 1e-10 x), and 2^-53 * |loss| / h
+            assert abs((up - loss(*args)) / (2 * h) - g[at]) < 1e-7, (k, at)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("R,C", [(9, 64), (5, 100), (3, 1024), (7, 1001), (3, 8192)])
+def test_layer_norm_of_arrays_that_start_anywhere(rt, R, C, dtype, offset):
+    """The results do not depend on where the arrays begin: views of rows start on any element."""
+    x, gain, bias, gy = _norm_inputs(R, C, dtype)
+    size = x.dtype.itemsize
+
+    def shifted(a):
+        d = Dev(np.concatenate([np.zeros(offset, dtype), a.reshape(-1), np.full(4, 9, dtype)]))
+        return d, ctypes.c_void_p(d.w.data + offset * size)
+    arrays = [shifted(a) for a in (x, gain, bias, gy)]
+    px, pg, pb, pgy = [p for (_d, p) in arrays]
+    outs = [shifted(np.full_like(a, 7)) for a in (x, x, gain, gain)]
+    call("cgtb_layer_norm_forward", code(dtype), px, R, C, pg, pb, 1e-5, outs[0][1])
+    call("cgtb_layer_norm_backward", code(dtype), px, pg, pgy, R, C, 1e-5, *[p for (_d, p) in outs[1:]])
+    bounds = ref.norm_bounds(x, gain, bias, gy, 1e-5)
+    wants = (ref.norm(x, gain, bias, 1e-5)[0],) + tuple(ref.norm_gradients(x, gain, gy, 1e-5))
+    for ((d, _p), want, bound) in zip(outs, wants, bounds):
+        flat = d.get()
+        assert (np.abs(flat[offset:offset + want.size].reshape(want.shape) - want) <= bound).all()
+        assert (flat[:offset] == 0).all() and (flat[offset + want.size:] == 9).all()      # nothing outside is written
+
+
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+def _dropout(x, p, seed, step, site, shift=0):
+    size = x.dtype.itemsize
+    d = Dev(np.concatenate([np.zeros(shift, x.dtype), x.reshape(-1)]))
+    y = Dev(np.full(x.size + shift + 8, 7, x.dtype))
+    state = Dev(np.array([seed, step], "i8"))
+    call("cgtb_dropout", code(x.dtype), ctypes.c_void_p(d.w.data + shift * size), x.size, p, state.ptr, site, ctypes.c_void_p(y.w.data + shift * size))
+    flat = y.get()
+    assert (flat[:shift] == 7).all() and (flat[shift + x.size:] == 7).all()
+    return flat[shift:shift + x.size].reshape(x.shape)
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 7, 8, 127, 1024, 4099, 65537, 1 << 20, (1 << 21) + 3])
+def test_dropout(rt, n, dtype):
+    x = np.random.RandomState(n).randn(n).astype(dtype)
+    for (p, seed, step, site, shift) in ((0.5, 0, 0, 0, 0), (0.1, 12345678901234567, 999, 3, 1), (0.93, -5, 2 ** 32 + 7, 1, 2), (1e-12, 1, 1, 1, 3), (0.0, 1, 1, 1, 0)):
+        assert np.array_equal(_dropout(x, p, seed, step, site, shift), ref.dropout(x, p, seed, step, site)), (p, seed, step, site, shift)
+
+
+def test_a_dropped_element_is_zero_whatever_it_was(rt):
+    x = np.random.RandomState(0).randn(4096).astype("f4")
+    keep = ref.kept(x.size, 0.5, 8, 2, 0)
+    x[~keep] = np.tile(np.array([np.inf, -np.inf, np.nan], "f4"), x.size)[:int((~keep).sum())]
+    y = _dropout(x, 0.5, 8, 2, 0)
+    assert (y[~keep] == 0).all() and np.array_equal(y[keep], 2 * x[keep])
+
+
+def test_dropout_of_its_own_memory(rt):
+    x = np.random.RandomState(0).randn(5001).astype("f4")
+    d, state = Dev(x), Dev(np.array([4, 5], "i8"))
+    call("cgtb_dropout", code("f4"), d.ptr, x.size, 0.3, state.ptr, 2, d.ptr)
+    assert np.array_equal(d.get(), ref.dropout(x, 0.3, 4, 5, 2))
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit rows and products
+# ------------------------------------------------------------------------------------------------
+def _quantize(x):
+    codes, scales = Dev(np.full((x.shape[0], -(-x.shape[1] // 16) * 16), 99, "i1")), Dev(np.full(x.shape[0], 7, "f4"))
+    d = Dev(x)
+    call("cgtb_quantize_rows", d.ptr, x.shape[0], x.shape[1], codes.ptr, scales.ptr)
+    return codes.get(), scales.get()
+
+
+def _same(got, want):
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1], equal_nan=True)
+
+
+@pytest.mark.parametrize("R,C", ROWS_COLS)
+def test_quantize_rows(rt, R, C):
+    x = _norm_inputs(R, C, "f4")[0]
+    _same(_quantize(x), ref.quantize(x))
+
+
+@pytest.mark.parametrize("C", [16, 40, 700, 3001, 17000])
+def test_quantize_rows_at_ties_and_at_the_ends_of_the_type(rt, C):
+    rs = np.random.RandomState(C)
+    x = np.zeros((16, C), "f4")
+    x[0] = rs.randint(-254, 255, size=C) / 2.0
+    x[0, C - 1] = 127                                            # every half is a tie
+    x[1] = x[0] * np.float32(2.0 ** -140)                        # denormal
+    x[2] = x[0] * np.float32(2.0 ** 120)
+    x[3] = rs.randn(C) * 1e-44
+    x[4] = rs.uniform(-1, 1, C) * 3.4e38
+    x[6, 0] = 1e-45
+    x[7, 0], x[8, C - 1], x[9, C // 2] = np.inf, np.nan, -np.inf
+    x[10, 3], x[10, 4] = -0.0, -3.0
+    base = rs.uniform(0.5, 1, 4).astype("f4")
+    for i in range(4):                                           # next to a tie on both sides
+        largest = base[i]
+        half = (np.arange(C) % 127 + 0.5) * float(largest) / 127
+        x[11 + i] = np.nextafter(half.astype("f4"), np.float32(4 * (i % 2))) if i < 2 else half.astype("f4")
+        x[11 + i, 0] = -largest
+    _same(_quantize(x), ref.quantize(x))
+
+
+def test_quantize_no_rows_and_no_columns(rt):
+    _same(_quantize(np.zeros((0, 33), "f4")), (np.zeros((0, 48), "i1"), np.zeros(0, "f4")))
+    _same(_quantize(np.zeros((5, 0), "f4")), (np.zeros((5, 0), "i1"), np.zeros(5, "f4")))
+
+
+PRODUCTS = [(1, 1, 16), (1, 1000, 784), (1, 4096, 4096), (2, 33, 48), (4, 10, 1008), (7, 129, 2000), (8, 256, 256), (9, 64, 144), (15, 100, 160),
+            (16, 128, 128), (17, 127, 112), (31, 500, 1024), (33, 65, 96), (64, 1000, 512), (65, 17, 4112), (100, 256, 32), (127, 1, 208), (128, 128, 128),
+            (129, 257, 400), (200, 300, 2064), (255, 1001, 1008), (256, 512, 64), (500, 96, 800), (1000, 10, 784), (1025, 515, 272), (3, 5000, 8192)]
+
+
+def _product(a, sa, b, sb, bias):
+    y = Dev(np.full((len(a), len(b)), 7, "f4"))
+    da, dsa, db, dsb = Dev(a), Dev(sa), Dev(b), Dev(sb)
+    dbias = Dev(bias) if bias is not None else None
+    call("cgtb_int8_product", da.ptr, dsa.ptr, db.ptr, dsb.ptr, dbias.ptr if bias is not None else None, len(a), len(b), a.shape[1], y.ptr)
+    return y.get()
+
+
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_int8_product(rt, M, N, K):
+    rs = np.random.RandomState(M + N + K)
+    a, b = rs.randint(-128, 128, (M, K)).astype("i1"), rs.randint(-128, 128, (N, K)).astype("i1")
+    sa, sb = rs.rand(M).astype("f4"), (rs.rand(N) * 0.01).astype("f4")
+    for bias in (None, rs.randn(N).astype("f4")):
+        want, bound = ref.product(a, sa, b, sb, bias)
+        off = np.abs(_product(a, sa, b, sb, bias) - want)
+        assert (off <= bound).all(), float((off / bound).max())
+
+
+@pytest.mark.parametrize("M,N", [(1, 3), (20, 5), (130, 3)])
+def test_int8_product_fills_its_sums(rt, M, N):
+    """The largest magnitudes at the longest row: 128 * 128 * 131056 is just below 2^31."""
+    K = 131056
+    a, b = np.full((M, K), -128, "i1"), np.full((N, K), -128, "i1")
+    b[1] = 127
+    one_m, one_n = np.ones(M, "f4"), np.ones(N, "f4")
+    want, bound = ref.product(a[:1], one_m[:1], b, one_n, None)
+    assert (np.abs(_product(a, one_m, b, one_n, None) - want) <= bound).all()
+
+
+def test_int8_product_of_rows_without_a_scale(rt):
+    """A row that could not be quantized (scale NaN) is NaN in the result, a row of zeros is the bias; the others are neither."""
+    rs = np.random.RandomState(0)
+    x = rs.randn(40, 100).astype("f4")
+    x[3], x[5, 7] = 0, np.inf
+    w, bias = rs.randn(50, 100).astype("f4"), rs.randn(50).astype("f4")
+    (a, sa), (b, sb) = _quantize(x), _quantize(w)
+    y = _product(a, sa, b, sb, bias)
+    assert np.isnan(y[5]).all() and np.array_equal(y[3], bias) and np.isfinite(np.delete(y, 5, 0)).all()
+
+
+def test_int8_product_without_rows_channels_or_terms(rt):
+    z = np.zeros
+    assert _product(z((0, 32), "i1"), z(0, "f4"), z((5, 32), "i1"), z(5, "f4"), None).shape == (0, 5)
+    assert _product(z((5, 32), "i1"), z(5, "f4"), z((0, 32), "i1"), z(0, "f4"), None).shape == (5, 0)
+    for M in (1, 40, 200):
+        bias = np.arange(3, dtype="f4")
+        assert np.array_equal(_product(z((M, 0), "i1"), z(M, "f4"), z((3, 0), "i1"), z(3, "f4"), bias), np.tile(bias, (M, 1)))
+
+
+def test_refused_calls_leave_the_library_usable(rt):
+    L = runtime.lib()
+    d = Dev(np.zeros((4, 32), "f4"))
+    c = Dev(np.zeros((4, 32), "i1"))
+    s = Dev(np.zeros(4, "f4"))
+    state = Dev(np.array([0, 0], "i8"))
+    off = ctypes.c_void_p(c.w.data + 1)
+    refused = [
+        ("cgtb_layer_norm_forward", (11, d.ptr, -1, 32, d.ptr, d.ptr, 1e-5, d.ptr)),
+        ("cgtb_layer_norm_forward", (11, d.ptr, 4, 32, d.ptr, d.ptr, -1e-5, d.ptr)),
+        ("cgtb_layer_norm_forward", (11, d.ptr, 4, 32, d.ptr, d.ptr, float("nan"), d.ptr)),
+        ("cgtb_layer_norm_forward", (7, d.ptr, 4, 32, d.ptr, d.ptr, 1e-5, d.ptr)),
+        ("cgtb_layer_norm_backward", (7, d.ptr, d.ptr, d.ptr, 4, 32, 1e-5, d.ptr, d.ptr, d.ptr)),
+        ("cgtb_dropout", (11, d.ptr, 32, 1.0, state.ptr, 0, d.ptr)),
+        ("cgtb_dropout", (11, d.ptr, 32, -0.1, state.ptr, 0, d.ptr)),
+        ("cgtb_dropout", (5, d.ptr, 32, 0.1, state.ptr, 0, d.ptr)),
+        ("cgtb_dropout", (11, d.ptr, -32, 0.1, state.ptr, 0, d.ptr)),
+        ("cgtb_quantize_rows", (d.ptr, -1, 32, c.ptr, s.ptr)),
+        ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, 4, 4, 24, d.ptr)),
+        ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, 4, 4, 131072, d.ptr)),
+        ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, -4, 4, 32, d.ptr)),
+        ("cgtb_int8_product", (off, s.ptr, c.ptr, s.ptr, None, 1, 1, 16, d.ptr)),
+    ]
+    for (name, args) in refused:
+        assert getattr(L, name)(*args) != 0 and name in runtime.last_error(), (name, args)
+    x = np.ones((2, 16), "f4")
+    _same(_quantize(x), ref.quantize(x))
+
+
+# ------------------------------------------------------------------------------------------------
+# in compiled functions
+# ------------------------------------------------------------------------------------------------
+def _shared(a):
+    return cgt.shared(a, fixed_shape_mask="all")
+
+
+@pytest.mark.parametrize("precision", ["single", "double"])
+def test_results_go_into_variables(rt, precision):
+    """Forward and backward results kept in variables, through captured replays and for new inputs."""
+    dt = "f4" if precision == "single" else "f8"
+    with cgt.scoped_update_config(precision=precision):
+        x, gain, bias, gy = [_shared(a) for a in _norm_inputs(50, 300, dt)]
+        y = nn.layer_norm(x, gain, bias)
+        news = [y] + core.pullback([y], [gy], [x, gain, bias])
+        outs = [_shared(np.zeros(s, dt)) for s in ((50, 300), (50, 300), (300,), (300,))]
+        f = cgt.function([], [], updates=list(zip(outs, news)))
+    assert not any(getattr(i.op, "opname", "").startswith("cast") for i in f.eg.instrs if hasattr(i, "op"))     # nothing is copied
+    for seed in (0, 0, 0, 0, 1, 2):
+        vals = _norm_inputs(50, 300, dt, seed)
+        for (v, a) in zip((x, gain, bias, gy), vals):
+            v.op.set_value(a)
+        f()
+        bounds = ref.norm_bounds(*vals, 1e-5)
+        wants = (ref.norm(*vals[:3], 1e-5)[0],) + tuple(ref.norm_gradients(vals[0], vals[1], vals[3], 1e-5))
+        for (o, want, bound) in zip(outs, wants, bounds):
+            assert (np.abs(o.op.get_value() - want) <= bound).all()
+
+
+def test_a_gradient_that_replaces_what_it_was_computed_from(rt):
+    """x := dx and gain := dgain: every result is formed from the old values."""
+    vals = _norm_inputs(20, 100, "f4")
+    x, gain, bias, gy = [_shared(a) for a in vals]
+    y = nn.layer_norm(x, gain, bias)
+    dx, dgain, dbias = core.pullback([y], [gy], [x, gain, bias])
+    cgt.function([], [], updates=[(x, dx), (gain, dgain), (gy, y), (bias, dbias)])()
+    bounds = ref.norm_bounds(*vals, 1e-5)
+    wants = (ref.norm(*vals[:3], 1e-5)[0],) + tuple(ref.norm_gradients(vals[0], vals[1], vals[3], 1e-5))
+    for (o, want, bound) in zip((gy, x, gain, bias), wants, bounds):
+        assert (np.abs(o.op.get_value() - want) <= bound).all()
+
+
+def test_every_step_drops_other_elements(rt):
+    """The masks of a captured step follow the stream's step; two dropouts of one stream differ; forward and backward agree."""
+    n = (70, 33)
+    xv = np.random.RandomState(0).randn(*n).astype("f4")
+    x = _shared(xv)
+    stream = nn.RandomStream(77)
+    a, b = nn.dropout(x, 0.4, stream), nn.dropout(x, 0.4, stream)
+    dx = core.pullback([a], [x * 3.0], [x])[0]
+    f = cgt.function([], [a, b, dx], updates=stream.updates())
+    for step in range(6):
+        got = f()
+        wants = [ref.dropout(xv, 0.4, 77, step, 0), ref.dropout(xv, 0.4, 77, step, 1), ref.dropout(xv * 3, 0.4, 77, step, 0)]
+        assert all(np.array_equal(g, w) for (g, w) in zip(got, wants)), step
+    assert list(stream.state.op.get_value()) == [77, 6]
+    g = cgt.function([], [a])            # without the update: the same elements in every call
+    assert all(np.array_equal(g()[0], ref.dropout(xv, 0.4, 77, 6, 0)) for _ in range(4))
+
+
+def _block(width, hidden, stream, seed):
+    """Affine(rectify(Affine(layer_norm(x)))) with dropout in training, as a network's block."""
+    np.random.seed(seed)
+    layers = [nn.LayerNorm(width), nn.Affine(width, hidden, weight_init=nn.XavierNormal()), nn.Affine(hidden, width, weight_init=nn.XavierNormal())]
+
+    def train(x):
+        h = nn.rectify(layers[1](layers[0](x)))
+        return x + nn.dropout(layers[2](nn.dropout(h, 0.2, stream)), 0.1, stream)
+
+    def predict(x):
+        return x + nn.Int8Affine(layers[2])(nn.rectify(nn.Int8Affine(layers[1])(layers[0](x))))
+    return layers, train, predict
+
+
+def _block_step(P, x, t, lr, seed, step):
+    """The block's training step in 64 bits: loss, new parameters."""
+    gain, bias, W1, b1, W2, b2 = P
+    R = len(x)
+    y, xh, rstd = ref.norm(x, gain, bias, 1e-5)
+    z = y @ W1 + b1
+    mask = z >= 0
+    keep1 = ref.kept(z.size, 0.2, seed, step, 0).reshape(z.shape) / 0.8
+    keep2 = ref.kept(x.size, 0.1, seed, step, 1).reshape(x.shape) / 0.9
+    h = z * mask * keep1
+    out = x + (h @ W2 + b2) * keep2
+    g = 2 * (out - t) / R * keep2
+    dh = g @ W2.T * keep1 * mask
+    dy = dh @ W1.T
+    grads = [(dy * xh).sum(0), dy.sum(0), y.T @ dh, dh.sum(0, keepdims=True), h.T @ g, g.sum(0, keepdims=True)]
+    return ((out - t) ** 2).sum() / R, [p - lr * d for (p, d) in zip(P, grads)], out
+
+
+@pytest.mark.parametrize("rows", [32, None])
+def test_a_block_is_trained_and_predicts_in_8_bits(rt, rows):
+    """Five steps against the formulas in 64 bits with the same masks, with a fixed and an open batch; then predictions in 8 bits
+    against the trained float32 weights."""
+    width, hidden, batch = 48, 120, 32
+    stream = nn.RandomStream(5)
+    layers, train, predict = _block(width, hidden, stream, 3)
+    X, T = cgt.matrix("X", fixed_shape=(rows, width)), cgt.matrix("T", fixed_shape=(rows, width))
+    loss = cgt.square(train(X) - T).sum() / float(batch)
+    params = [layers[0].gain, layers[0].bias, layers[1].weight, layers[1].bias, layers[2].weight, layers[2].bias]
+    f = cgt.function([X, T], [loss], updates=nn.sgd(loss, params, 0.02) + stream.updates())
+    P = [p.op.get_value().astype("f8") for p in params]
+    rs = np.random.RandomState(0)
+    for step in range(5):
+        x, t = rs.randn(batch, width).astype("f4"), rs.randn(batch, width).astype("f4")
+        got = f(x, t)[0]
+        want, P, _out = _block_step(P, x.astype("f8"), t.astype("f8"), 0.02, 5, step)
+        # sums of up to 4000 float32 terms; a rectifier's argument next to 0 may change sides, which moves its gradient's terms by as little
+        np.testing.assert_allclose(got, want, rtol=1e-5)
+        for (p, w) in zip(params, P):
+            np.testing.assert_allclose(p.op.get_value(), w, rtol=1e-4, atol=2e-5)
+    # 8-bit rows and weights: every factor is off by at most half a code, 1 / 254 of its row's largest magnitude
+    x = rs.randn(batch, width).astype("f4")
+    q = cgt.function([X], [predict(X)])
+    y, W1, W2 = ref.norm(x, *[p.astype("f8") for p in P[:2]], 1e-5)[0], P[2], P[4]
+    z = np.maximum(y @ W1 + P[3], 0)
+    exact = x + z @ W2 + P[5]
+
+    def spread(a, W, e):   # bound on the error of a.W with a off by e
+        half_a = np.abs(a).max(1, keepdims=True) / 254 + e
+        half_w = np.abs(W).max(0) / 254
+        return half_a * np.abs(W).sum(0) + (np.abs(a) + half_a).sum(1, keepdims=True) * half_w
+    bound = spread(z, W2, spread(y, W1, 1e-6).max(1, keepdims=True) * 1.01) + 1e-4
+    for _ in range(4):
+        assert (np.abs(q(x)[0] - exact) <= bound).all()
+
+
+def test_int8_affine_follows_numpy(rt):
+    """The layer's result from the codes that numpy makes, for batches of several sizes through one function."""
+    np.random.seed(1)
+    layer = nn.Affine(70, 33, weight_init=nn.XavierNormal(), bias_init=nn.IIDGaussian())
+    X = cgt.matrix("X", fixed_shape=(None, 70))
+    f = cgt.function([X], [nn.Int8Affine(layer)(X)])
+    b, sb = ref.quantize(layer.weight.op.get_value().T.copy())
+    for rows in (1, 5, 5, 5, 5, 40, 200, 1):
+        x = np.random.randn(rows, 70).astype("f4")
+        want, bound = ref.product(*ref.quantize(x), b, sb, layer.bias.op.get_value()[0])
+        assert (np.abs(f(x)[0] - want) <= bound).all()
+
+
+def test_arguments_that_do_not_fit_are_errors(rt):
+    x = cgt.matrix("x")
+    g = _shared(np.ones(10, "f4"))
+    f = cgt.function([x], [nn.layer_norm(x, g, g)])
+    with pytest.raises(runtime.BackendError, match="one value for each"):
+        f(np.ones((3, 11), "f4"))
+    assert f(np.ones((3, 10), "f4"))[0].shape == (3, 10)
+    codes, scales = nn.quantize_rows(x)
+    w = _shared(np.ones((4, 32), "i1"))
+    f = cgt.function([x], [nn.int8_product(codes, scales, w, _shared(np.ones(4, "f4")))])
+    with pytest.raises(runtime.BackendError, match="rows of one length"):
+        f(np.ones((3, 10), "f4"))
+    assert f(np.ones((3, 20), "f4"))[0].shape == (3, 4)
+
+
+def test_arrays_of_other_ranks(rt):
+    rs = np.random.RandomState(0)
+    v, t = rs.randn(24).astype("f4"), rs.randn(3, 4, 24).astype("f4")
+    gain, bias = rs.randn(24).astype("f4"), rs.randn(24).astype("f4")
+    a, b = cgt.vector("a"), cgt.tensor3("b")
+    stream = nn.RandomStream(1)
+    f = cgt.function([a, b], [nn.layer_norm(a, _shared(gain), _shared(bias)), nn.layer_norm(b, _shared(gain), _shared(bias)), nn.dropout(b, 0.5, stream)])
+    ya, yb, d = f(v, t)
+    for (got, x) in ((ya, v[None]), (yb, t.reshape(-1, 24))):
+        assert (np.abs(got.reshape(x.shape) - ref.norm(x, gain, bias, 1e-5)[0]) <= ref.norm_bounds(x, gain, bias, None, 1e-5)).all()
+    assert np.array_equal(d, ref.dropout(t, 0.5, 1, 0, 0))
