@@ -15,11 +15,11 @@ namespace {
 
 constexpr int kRows = 128;          // rows of a per tile: the tensor core's M
 constexpr int kDepth = 128;         // codes of K per stage: one 128-byte swizzle row
-constexpr int kMaxStages = 8;
-constexpr int kEpilogueWarps = 4;   // one for each quarter of the accumulator's lanes
-constexpr int kThreads = kEpilogueWarps * 32 + 64;
-constexpr int kPitch = 36;          // floats per row of an epilogue warp's 32 x 32 block: 16-byte accesses without bank conflicts
+constexpr int kMaxStages = 32;
+constexpr int kEpilogueWarps = 8;   // two for each quarter of the accumulator's lanes
+constexpr int kThreads = (kEpilogueWarps + 3) * 32;   // and a warp for the MMAs, one for the loads of a, one for those of b
 constexpr int kGroup = 16;          // row tiles that are walked together: their codes and the weights stay in L2
+constexpr int kSlotBytes = kRows * 32 * 4;   // 32 columns of a tile's partial sums, column by column
 
 struct Params {
   const float *sa, *sb, *bias;
@@ -29,6 +29,8 @@ struct Params {
   int mtiles, ntiles;
   long total;
   int vec;
+  int split, split_log;             // CTAs of a cluster that share a tile, a power of two
+  int block_offset;                 // of the epilogue's blocks in shared memory
   int* err;
 };
 
@@ -56,47 +58,133 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, in
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// The epilogue's wait, bounded and abortable: one lane polls, and sleeps in between.
+__device__ __forceinline__ bool wait_sleeping(uint32_t bar, uint32_t parity, const volatile int* abort_flag, int lane) {
+  int ok = 1;
+  if (lane == 0 && !mbar_try(bar, parity)) {
+    const long long t0 = clock64();
+    ok = 0;
+    for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+      __nanosleep(64);
+      if (mbar_try(bar, parity)) { ok = 1; break; }
+      if ((spin & 15u) == 15u && (*abort_flag || clock64() - t0 > kWaitCycles)) break;
+    }
+  }
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  if (ok) (void)mbar_try(bar, parity);   // every lane observes the phase itself
+  return ok != 0;
 }
 
-// One CTA per SM walks tiles of 128 x BN results. One thread issues the TMA loads of a ring of stages (128 codes of K: 128 bytes
-// of every row of a and of b), one thread the MMAs (four of K = 32 per stage) into one of two accumulators in TMEM, four warps
-// turn the other accumulator into results meanwhile. Rows and codes beyond the operands arrive as zeros; what a box that is
-// shorter than 128 rows leaves in its stage feeds rows that are not stored.
+// Word offset of quad q of row `row` in a warp's 32 x 16 block: 16-byte accesses by rows and by quads without bank conflicts
+__device__ __forceinline__ int block_at(int row, int q) { return row * 16 + 4 * (q ^ ((row >> 1) & 3)); }
+
+__device__ __forceinline__ float4 finished(float4 v, float4 s, float4 b, bool bias) {
+  if (bias) return make_float4(v.x * s.x + b.x, v.y * s.y + b.y, v.z * s.z + b.z, v.w * s.w + b.w);
+  return make_float4(v.x * s.x, v.y * s.y, v.z * s.z, v.w * s.w);
+}
+
+// 16 columns of a warp's 32 rows: lane l holds row l's sums. They are scaled by the row, turned through shared memory, scaled by
+// the column and stored, eight rows of 64 bytes at a time. `columns`: the scales of the 16 columns, 256 floats on their biases.
+__device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[16], float row_scale, long m0, long n0, float* block, const float* columns,
+                                            int lane) {
+  const int nrows = (int)(p.M - m0 < 32 ? p.M - m0 : 32);
+  __syncwarp();   // the block's previous content has been read
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<float4*>(block + block_at(lane, q)) =
+        make_float4((float)(int)r[4 * q] * row_scale, (float)(int)r[4 * q + 1] * row_scale, (float)(int)r[4 * q + 2] * row_scale,
+                    (float)(int)r[4 * q + 3] * row_scale);
+  const bool bias = p.bias != nullptr;
+  __syncwarp();
+  if (p.vec) {      // N a multiple of four
+    const int q = lane & 3, row0 = lane >> 2;
+    if (n0 + 4 * q < p.N) {
+      const float4 s = *reinterpret_cast<const float4*>(columns + 4 * q), b = *reinterpret_cast<const float4*>(columns + 256 + 4 * q);
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float4*>(block + block_at(row0 + 8 * i, q));
+      float* dst = p.y + (m0 + row0) * p.N + n0 + 4 * q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row0 + 8 * i < nrows) *reinterpret_cast<float4*>(dst + 8 * i * p.N) = finished(v[i], s, b, bias);
+    }
+  } else {
+    const int c = lane & 15;
+    if (n0 + c < p.N) {
+      const float s = columns[c], b = columns[256 + c];
+      float* dst = p.y + (m0 + (lane >> 4)) * p.N + n0 + c;
+#pragma unroll 4
+      for (int row = lane >> 4; row < nrows; row += 2, dst += 2 * p.N) {
+        const float v = block[block_at(row, c >> 2) + (c & 3)];
+        *dst = bias ? v * s + b : v * s;
+      }
+    }
+  }
+}
+// the scales and biases of a tile's columns, brought to shared memory while the tile's sums are formed; `it`: two places
+__device__ __forceinline__ const float* stage_columns(const Params& p, float* columns, uint32_t it, long n0, int tid) {
+  float* to = columns + (it & 1u) * 512;
+  const long n = n0 + tid;
+  if (tid < p.BN) {
+    to[tid] = n < p.N ? p.sb[n] : 0.f;
+    to[256 + tid] = n < p.N && p.bias ? p.bias[n] : 0.f;
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
+  return to;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote_address(uint32_t local, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ void store_remote(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+
+// One CTA per SM walks tiles of 128 x BN results. One thread issues the TMA loads of a, one those of b, into a ring of stages (128
+// codes of K: 128 bytes of every row), one thread the MMAs (four of K = 32 per stage) into one of two accumulators in TMEM, eight
+// warps turn the other accumulator into results meanwhile. Rows and codes beyond the operands arrive as zeros. With fewer than
+// 128 rows the box of a is as short as they are, and the MMAs read on into what lies behind it (at the ring's end the epilogue's
+// blocks, 16 KB like a full box): whole numbers that only reach rows which are not stored.
+//
+// SPLIT: fewer tiles than SMs. The CTAs of a cluster share a tile, each sums over a slice of K; then every CTA sends its partial
+// sums to the CTA that finishes their columns (chunk c of 16 columns: CTA c % split), through distributed shared memory, and adds
+// what it receives (whole numbers: in any order). An MMA takes a hundred cycles however narrow the tile, so a tile stays wide
+// and K is split.
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(16) float columns[2 * 512];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t a_stage = kRows * kDepth, stage_bytes = a_stage + (uint32_t)p.BN * kDepth;
+  const uint32_t a_stage = (uint32_t)p.a_bytes, stage_bytes = a_stage + (uint32_t)p.BN * kDepth;
   volatile int* abortp = &abort_flag;
-  const int nkb = (int)((p.K + kDepth - 1) / kDepth);
+  const uint32_t rank = SPLIT ? cluster_rank() : 0u;
+  const long t_first = SPLIT ? blockIdx.x >> p.split_log : blockIdx.x, t_step = SPLIT ? p.total : gridDim.x;   // SPLIT: one tile
+  const int nkb_all = (int)((p.K + kDepth - 1) / kDepth), kb_first = SPLIT ? ((int)rank * nkb_all) >> p.split_log : 0;
+  const int nkb = (SPLIT ? (((int)rank + 1) * nkb_all) >> p.split_log : nkb_all) - kb_first;
 
+  if (tid < p.stages) {
+    mbar_init(smem_u32(&full[tid]), 2);
+    mbar_init(smem_u32(&empty[tid]), 1);
+  }
   if (tid == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
-    }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&acc_full[b]), 1);
       mbar_init(smem_u32(&acc_empty[b]), kEpilogueWarps);
     }
     abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
   }
+  if (warp == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");   // all barriers are this warp's
   if (warp == kEpilogueWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"((uint32_t)p.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -105,58 +193,34 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
+  const int quarter = warp & 3, half = warp >> 2;
+  float* block = reinterpret_cast<float*>(smem + p.block_offset) + warp * 512;
+  const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+  bool ok = true;
+  float row_scale = 0.f;            // SPLIT: kept for the end
 
   if (warp < kEpilogueWarps) {
-    float* block = reinterpret_cast<float*>(smem + (size_t)p.stages * stage_bytes) + warp * 32 * kPitch;
     uint32_t it = 0;
-    for (long t = blockIdx.x; t < p.total; t += gridDim.x, ++it) {
+    for (long t = t_first; t < p.total; t += t_step, ++it) {
       const Tile c = tile_of(p, t);
       const uint32_t buf = it & 1u;
-      bool ok = mbar_wait_or_abort(smem_u32(&acc_full[buf]), (it >> 1) & 1u, abortp);
-      ok = __all_sync(0xffffffffu, ok);
+      const long m0 = c.m0 + quarter * 32;
+      row_scale = m0 + lane < p.M ? p.sa[m0 + lane] : 0.f;
+      const float* scales = stage_columns(p, columns, it, c.n0, tid);
+      ok = wait_sleeping(smem_u32(&acc_full[buf]), (it >> 1) & 1u, abortp, lane);
       if (!ok) {
         *abortp = 1;
         if (lane == 0) { *(volatile int*)p.err = 3; __threadfence_system(); }
-        break;
       }
+      if (SPLIT) break;
+      // the epilogue warps go on together: they meet at a barrier in every tile
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
+      if (*abortp) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const long mrow = c.m0 + warp * 32 + lane;      // the row of this lane's accumulators
-      const float scale = mrow < p.M ? p.sa[mrow] : 0.f;
-      const long mfirst = c.m0 + warp * 32;
-      const int nrows = (int)(p.M - mfirst < 32 ? p.M - mfirst : 32);
-      for (int ch = 0; ch < p.BN / 32; ++ch) {
-        uint32_t r[32];
-        tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + buf * (uint32_t)p.BN + (uint32_t)ch * 32u, r);
-        const long n0 = c.n0 + ch * 32;
-        __syncwarp();   // the block's previous content has been read
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<float4*>(block + lane * kPitch + 4 * q) =
-              make_float4((float)(int)r[4 * q] * scale, (float)(int)r[4 * q + 1] * scale, (float)(int)r[4 * q + 2] * scale, (float)(int)r[4 * q + 3] * scale);
-        __syncwarp();
-        if (p.vec) {      // N a multiple of four: a warp stores four rows of 128 bytes at a time
-          const int q = lane & 7;
-          const long n = n0 + 4 * q;
-          if (n < p.N) {
-            const float4 s = make_float4(p.sb[n], p.sb[n + 1], p.sb[n + 2], p.sb[n + 3]);
-            const float4 b = p.bias ? make_float4(p.bias[n], p.bias[n + 1], p.bias[n + 2], p.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int row = lane >> 3; row < nrows; row += 4) {
-              const float4 v = *reinterpret_cast<const float4*>(block + row * kPitch + 4 * q);
-              *reinterpret_cast<float4*>(p.y + (mfirst + row) * p.N + n) =
-                  p.bias ? make_float4(v.x * s.x + b.x, v.y * s.y + b.y, v.z * s.z + b.z, v.w * s.w + b.w)
-                         : make_float4(v.x * s.x, v.y * s.y, v.z * s.z, v.w * s.w);
-            }
-          }
-        } else {
-          const long n = n0 + lane;
-          if (n < p.N) {
-            const float s = p.sb[n], b = p.bias ? p.bias[n] : 0.f;
-            for (int row = 0; row < nrows; ++row) {
-              const float v = block[row * kPitch + lane];
-              p.y[(mfirst + row) * p.N + n] = p.bias ? v * s + b : v * s;
-            }
-          }
-        }
+      for (int ch = half; m0 < p.M && ch < p.BN / 16; ch += 2) {
+        uint32_t r[16];
+        tmem_ld16(lanes + buf * (uint32_t)p.BN + (uint32_t)ch * 16u, r);
+        store_chunk(p, r, row_scale, m0, c.n0 + ch * 16, block, scales + ch * 16, lane);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -164,61 +228,103 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     }
   } else if (warp == kEpilogueWarps) {
     // MMA issuer
-    const uint32_t idesc = idesc_int8(p.BN);
-    bool ok = true;
+    const uint32_t idesc = idesc_int8(p.BN), base = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+    const uint64_t da0 = make_desc(base), db0 = make_desc(base + a_stage);
+    const uint32_t step = stage_bytes >> 4;
     if (elect_one()) {
-      int s = 0;
-      uint32_t phase = 0, it = 0;
-      for (long t = blockIdx.x; t < p.total && ok; t += gridDim.x, ++it) {
+      uint32_t s = 0, phase = 0, it = 0;
+      for (long t = t_first; t < p.total && ok; t += t_step, ++it) {
         const uint32_t buf = it & 1u;
         ok = mbar_wait_or_abort(smem_u32(&acc_empty[buf]), ((it >> 1) & 1u) ^ 1u, abortp);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + buf * (uint32_t)p.BN;
         for (int kb = 0; kb < nkb; ++kb) {
-          ok = mbar_wait_or_abort(smem_u32(&full[s]), phase, abortp);
+          ok = mbar_wait_or_abort(full0 + 8u * s, phase, abortp);   // what TMA wrote needs no further fence
           if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t base = smem_u32(smem + (size_t)s * stage_bytes);
-          const uint64_t da = make_desc(base), db = make_desc(base + a_stage);
-#pragma unroll
-          for (int kk = 0; kk < kDepth / 32; ++kk)     // 32 codes: 32 bytes further inside the swizzle row
-            mma_int8(d, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), idesc, (kb | kk) ? 1u : 0u);
-          mma_commit(smem_u32(&empty[s]));
-          if (++s == p.stages) { s = 0; phase ^= 1u; }
+          const uint64_t da = da0 + s * step, db = db0 + s * step;
+          mma_int8(d, da, db, idesc, kb > 0);                  // 32 codes: 32 bytes further inside the swizzle row
+          mma_int8(d, da + 2, db + 2, idesc, 1u);
+          mma_int8(d, da + 4, db + 4, idesc, 1u);
+          mma_int8(d, da + 6, db + 6, idesc, 1u);
+          mma_commit(empty0 + 8u * s);
+          if (++s == (uint32_t)p.stages) { s = 0; phase ^= 1u; }
         }
         if (ok) mma_commit(smem_u32(&acc_full[buf]));
       }
       if (!ok) { *abortp = 1; *(volatile int*)p.err = 4; __threadfence_system(); }
     }
     __syncwarp();
-  } else if (lane == 0) {
-    // TMA producer
-    long issued = 0;
-    bool ok = true;
-    int s = 0;
-    uint32_t phase = 0;
-    const uint32_t tx = (uint32_t)p.a_bytes + (uint32_t)p.BN * kDepth;
-    for (long t = blockIdx.x; t < p.total && ok; t += gridDim.x) {
-      const Tile c = tile_of(p, t);
-      for (int kb = 0; kb < nkb; ++kb) {
-        ok = mbar_wait_or_abort(smem_u32(&empty[s]), phase ^ 1u, abortp);
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + (size_t)s * stage_bytes);
-        mbar_arrive_expect_tx(bar, tx);
-        load_2d(dst, &map_a, kb * kDepth, (int)c.m0, bar);
-        load_2d(dst + a_stage, &map_b, kb * kDepth, (int)c.n0, bar);
-        ++issued;
-        if (++s == p.stages) { s = 0; phase ^= 1u; }
+  } else {
+    if (elect_one()) {
+      // TMA producers: one thread for the boxes of a, one for those of b
+      const bool is_b = warp == kEpilogueWarps + 2;
+      const CUtensorMap* map = is_b ? &map_b : &map_a;
+      const uint32_t tx = is_b ? (uint32_t)p.BN * kDepth : a_stage, dst0 = smem_u32(smem) + (is_b ? a_stage : 0u);
+      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
+      uint32_t issued = 0, s = 0, phase = 1;
+      for (long t = t_first; t < p.total && ok; t += t_step) {
+        const Tile c = tile_of(p, t);
+        const int row = (int)(is_b ? c.n0 : c.m0);
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_or_abort(empty0 + 8u * s, phase, abortp);
+          if (!ok) break;
+          mbar_arrive_expect_tx(full0 + 8u * s, tx);
+          load_2d(dst0 + s * stage_bytes, map, (kb_first + kb) * kDepth, row, full0 + 8u * s);
+          ++issued;
+          if (++s == (uint32_t)p.stages) { s = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok || *abortp) {
+        *abortp = 1;
+        *(volatile int*)p.err = 5;
+        __threadfence_system();
+        // copies already issued still write this CTA's shared memory: wait (bounded) until they have landed
+        const uint32_t stages = (uint32_t)p.stages;
+        for (uint32_t j = (issued > stages ? issued - stages : 0u); j != issued; ++j) mbar_wait(full0 + 8u * (j % stages), (j / stages) & 1u);
       }
     }
-    if (!ok || *abortp) {
-      *abortp = 1;
-      *(volatile int*)p.err = 5;
-      __threadfence_system();
-      // copies already issued still write this CTA's shared memory: wait (bounded) until they have landed
-      for (long j = (issued > p.stages ? issued - p.stages : 0); j < issued; ++j)
-        mbar_wait(smem_u32(&full[j % p.stages]), (uint32_t)(j / p.stages) & 1u);
+    __syncwarp();
+  }
+
+  if (SPLIT) {
+    // Every CTA passes both barriers, whatever happened to its waits. Behind the first one all MMAs of the cluster have run and
+    // the rings are free: they take the partial sums, one slot of 128 rows for each (sender, chunk of 32 columns).
+    cluster_sync();
+    const Tile c = tile_of(p, t_first);
+    const long m0 = c.m0 + quarter * 32;
+    const bool takes_part = warp < kEpilogueWarps && ok && m0 < p.M;
+    const int chunks = p.BN / 32, mine = (chunks + p.split - 1) >> p.split_log, row = quarter * 32 + lane;
+    const uint32_t half_columns = (uint32_t)half * 16u;       // a warp takes 16 of a chunk's 32 columns
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (takes_part) {
+      const uint32_t slots = smem_u32(smem) + half_columns * (kRows * 4) + (uint32_t)row * 4u;
+      for (int ch = 0; ch < chunks; ++ch) {
+        const uint32_t owner = (uint32_t)(ch & (p.split - 1));
+        if (owner == rank) continue;
+        uint32_t r[16];
+        tmem_ld16(lanes + (uint32_t)ch * 32u + half_columns, r);
+        const uint32_t sender = rank < owner ? rank : rank - 1u;
+        const uint32_t at = remote_address(slots + (sender * (uint32_t)mine + (uint32_t)(ch >> p.split_log)) * kSlotBytes, owner);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) store_remote(at + (uint32_t)(j * kRows * 4), r[j]);   // a warp stores 128 bytes of a column
+      }
+    }
+    cluster_sync();
+    if (takes_part) {
+      for (int i = 0; i < mine; ++i) {
+        const int ch = (i << p.split_log) + (int)rank;
+        if (ch >= chunks) break;
+        uint32_t r[16];
+        tmem_ld16(lanes + (uint32_t)ch * 32u + half_columns, r);
+        for (int sender = 0; sender + 1 < p.split; ++sender) {
+          const uint32_t* from = reinterpret_cast<const uint32_t*>(smem + (size_t)(sender * mine + i) * kSlotBytes) + half_columns * kRows + row;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] += from[j * kRows];
+        }
+        const int col = ch * 32 + (int)half_columns;
+        store_chunk(p, r, row_scale, m0, c.n0 + col, block, columns + col, lane);
+      }
     }
   }
 
@@ -259,23 +365,58 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
   p.sa = sa; p.sb = sb; p.bias = bias; p.y = y;
   p.M = M; p.N = N; p.K = K;
   p.mtiles = (int)cgtb_ceil_div(M, kRows);
-  // the widest tile that still gives every SM one
-  p.BN = 256;
-  while (p.BN > 32 && p.mtiles * cgtb_ceil_div(N, p.BN) < rt().sm_count) p.BN /= 2;
+  // Widths and splits, by what they cost in cycles (measured): a stage takes 400 or, wide, two for each column; tiles follow each
+  // other on an SM; a cluster's two barriers and its last step take 3000, what a CTA sends goes at 12 bytes a cycle. At
+  // 128 x 4096 x 4096 a width of 32 takes PAUSE us, 128 in clusters of four PAUSE us.
+  const int nkb = (int)cgtb_ceil_div(K, kDepth), sms = rt().sm_count;
+  long best = -1;
+  for (int bn = 256; bn >= 32; bn /= 2) {
+    if (bn > 32 && bn / 2 >= N) continue;
+    const long tiles = p.mtiles * cgtb_ceil_div(N, bn), rows = std::min<long>(M, kRows);
+    for (int log = 0; log <= 2 && (1 << log) <= nkb; ++log) {      // clusters of eight leave a fifth of the SMs without work
+      const int split = 1 << log;
+      if (split > 1 && tiles * split > sms) break;
+      const long waves = cgtb_ceil_div(tiles * split, sms), blocks = cgtb_ceil_div(nkb, split);
+      const long cost = waves * (blocks * std::max(400, 2 * bn) + 500) + (split > 1 ? 3000 + rows * bn * 4 * (split - 1) / split / 12 : 0);
+      if (best < 0 || cost < best) { best = cost; p.BN = bn; p.split = split; p.split_log = log; }
+    }
+  }
   p.ntiles = (int)cgtb_ceil_div(N, p.BN);
   p.total = (long)p.mtiles * p.ntiles;
-  p.tmem_cols = 2 * p.BN;
+  p.tmem_cols = (p.split > 1 ? 1 : 2) * p.BN;
   const int a_rows = (int)std::min<long>(kRows, cgtb_ceil_div(M, 8) * 8);
   p.a_bytes = a_rows * kDepth;
   p.vec = N % 4 == 0 && ((uintptr_t)y & 15) == 0;
-  const int stage_bytes = (kRows + p.BN) * kDepth, epilogue = kEpilogueWarps * 32 * kPitch * 4;
-  p.stages = std::min(kMaxStages, (225 * 1024 - 1024 - epilogue) / stage_bytes);
-  const int smem = 1024 + p.stages * stage_bytes + epilogue;
+  const int stage_bytes = p.a_bytes + p.BN * kDepth, epilogue = kEpilogueWarps * 512 * 4;
+  p.stages = std::min(kMaxStages, (220 * 1024 - 1024 - epilogue) / stage_bytes);
+  if (p.split > 1) p.stages = std::min(p.stages, (int)cgtb_ceil_div(nkb, p.split));
+  const int slots = (p.split - 1) * (int)cgtb_ceil_div(p.BN / 32, p.split) * kSlotBytes;
+  p.block_offset = std::max(p.stages * stage_bytes, slots);
+  const int smem = 1024 + p.block_offset + epilogue;
   CUtensorMap map_a, map_b;
   if (!encode(&map_a, a, M, K, a_rows) || !encode(&map_b, b, N, K, p.BN)) return fail("cgtb_int8_product: no tensor map for %ld x %ld x %ld", M, N, K);
-  static const cudaError_t attribute = cudaFuncSetAttribute(int8_product_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+  static const cudaError_t attribute = [] {
+    const cudaError_t e = cudaFuncSetAttribute(int8_product_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(int8_product_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  }();
   if (attribute != cudaSuccess) return fail("cgtb_int8_product: %s", cudaGetErrorString(attribute));
-  CGTB_LAUNCH(int8_product_tc_kernel, (unsigned)std::min<long>(p.total, rt().sm_count), kThreads, smem, map_a, map_b, p);
+  if (p.split > 1) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(p.total * p.split));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = rt().stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    CGTB_CUDA_TRY(cudaLaunchKernelEx(&config, int8_product_tc_kernel<true>, map_a, map_b, p));
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  } else {
+    CGTB_LAUNCH(int8_product_tc_kernel<false>, (unsigned)std::min<long>(p.total, sms), kThreads, smem, map_a, map_b, p);
+  }
   CGTB_CHECK_LAUNCH("int8_product");
   return 0;
 }
