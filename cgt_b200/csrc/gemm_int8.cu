@@ -421,19 +421,87 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
   return 0;
 }
 
-// Few rows: one thread per result
-__global__ void __launch_bounds__(256) int8_product_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
-                                                           const float* __restrict__ sb, const float* __restrict__ bias, long M, long N, long K,
-                                                           float* __restrict__ y) {
+// Few rows (one token at a time, up to eight): bound by the bytes of the weights. WARPS warps share an output channel, each lane
+// takes 16 codes of the channel's row at a time, four such loads in flight, and multiplies them with the codes of ROWS rows,
+// which come from the L1 cache; whole numbers are added by redux, in any order.
+template <int ROWS, int WARPS>
+__global__ void __launch_bounds__(256) int8_product_rows_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
+                                                                const float* __restrict__ sb, const float* __restrict__ bias, int M, long N, long K,
+                                                                float* __restrict__ y) {
+  __shared__ int part[8][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = warp % WARPS;
+  const long n = (long)blockIdx.x * (8 / WARPS) + warp / WARPS;
+  int sums[ROWS];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) sums[m] = 0;
+  if (n < N) {
+    const int8_t* w = b + n * K;
+    long k = (slice * 32 + lane) * 16;
+    constexpr long kStep = WARPS * 32 * 16;
+    for (; k + 3 * kStep < K; k += 4 * kStep) {
+      int4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __ldg(reinterpret_cast<const int4*>(w + k + u * kStep));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m) {
+          if (m >= M) break;
+          const int4 x = __ldg(reinterpret_cast<const int4*>(a + m * K + k + u * kStep));
+          sums[m] = __dp4a(v[u].x, x.x, __dp4a(v[u].y, x.y, __dp4a(v[u].z, x.z, __dp4a(v[u].w, x.w, sums[m]))));
+        }
+    }
+    for (; k < K; k += kStep) {
+      const int4 v = __ldg(reinterpret_cast<const int4*>(w + k));
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        if (m >= M) break;
+        const int4 x = __ldg(reinterpret_cast<const int4*>(a + m * K + k));
+        sums[m] = __dp4a(v.x, x.x, __dp4a(v.y, x.y, __dp4a(v.z, x.z, __dp4a(v.w, x.w, sums[m]))));
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) sums[m] = __reduce_add_sync(0xffffffffu, sums[m]);
+  if (WARPS > 1) {
+    if (lane == 0)
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) part[warp][m] = sums[m];
+    __syncthreads();
+    if (slice != 0) return;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) sums[m] += part[warp + i][m];
+  }
+  if (n >= N) return;
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+    if (lane == m && m < M) {
+      const float v = (float)sums[m] * sa[m] * sb[n];
+      y[m * N + n] = bias ? v + bias[n] : v;
+    }
+}
+
+template <int ROWS>
+int product_rows(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K, float* y) {
+  // as many warps for a channel as there are slices of 512 codes in its row, while the SMs are not full of warps
+  const long full = (long)rt().sm_count * 32;
+  const int warps = K > 2048 && N * 4 <= full ? 8 : K > 512 && N <= full ? 2 : 1;
+  const unsigned grid = (unsigned)cgtb_ceil_div(N, 8 / warps);
+  if (warps == 8) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 8>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
+  else if (warps == 2) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 2>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
+  else CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 1>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
+  CGTB_CHECK_LAUNCH("int8_product");
+  return 0;
+}
+
+// No terms: y = bias
+__global__ void __launch_bounds__(256) int8_product_empty_kernel(const float* __restrict__ sa, const float* __restrict__ sb, const float* __restrict__ bias,
+                                                                 long M, long N, float* __restrict__ y) {
   for (long o = blockIdx.x * 256L + threadIdx.x; o < M * N; o += gridDim.x * 256L) {
-    const long m = o / N, n = o - m * N;
-    const int* pa = (const int*)(a + m * K);
-    const int* pb = (const int*)(b + n * K);
-    int s = 0;
-    for (long k = 0; k < K / 4; ++k) s = __dp4a(pa[k], pb[k], s);
-    float v = (float)s * sa[m] * sb[n];
-    if (bias) v += bias[n];
-    y[o] = v;
+    const float v = 0.f * sa[o / N] * sb[o % N];
+    y[o] = bias ? v + bias[o % N] : v;
   }
 }
 
@@ -447,9 +515,14 @@ CGTB_API int cgtb_int8_product(const int8_t* a, const float* sa, const int8_t* b
   if (((uintptr_t)a | (uintptr_t)b) & 15) return fail("cgtb_int8_product: the codes have to start on a 16-byte boundary");
   if (M > 0x7fffffffL || N > 0x7fffffffL) return fail("cgtb_int8_product: more than 2^31 - 1 rows or channels");
   if (M == 0 || N == 0) return 0;
-  if (M > 8 && K > 0) return product_tc(a, sa, b, sb, bias, M, N, K, y);
-  const long blocks = cgtb_ceil_div(M * N, 256);
-  CGTB_LAUNCH(int8_product_kernel, (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), 256, 0, a, sa, b, sb, bias, M, N, K, y);
-  CGTB_CHECK_LAUNCH("int8_product");
-  return 0;
+  if (K == 0) {
+    const long blocks = cgtb_ceil_div(M * N, 256);
+    CGTB_LAUNCH(int8_product_empty_kernel, (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), 256, 0, sa, sb, bias, M, N, y);
+    CGTB_CHECK_LAUNCH("int8_product");
+    return 0;
+  }
+  if (M == 1) return product_rows<1>(a, sa, b, sb, bias, M, N, K, y);
+  if (M <= 4) return product_rows<4>(a, sa, b, sb, bias, M, N, K, y);
+  if (M <= 8) return product_rows<8>(a, sa, b, sb, bias, M, N, K, y);
+  return product_tc(a, sa, b, sb, bias, M, N, K, y);
 }

@@ -2,25 +2,82 @@
 // sm_100a.
 #include "runtime.h"
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 using namespace cgtb;
 
 namespace {
 
-constexpr int kRowThreads = 256;
+// ================================================================================================
+// Teams. A team of TEAM threads holds one row in its registers, E = N * VEC elements in each thread: element
+// (i * TEAM + thread) * VEC + v, so that a team reads and writes consecutive addresses, 16 bytes a thread where rows start on
+// 16-byte boundaries (VEC * sizeof(T) = 16) and element by element otherwise. TEAM is the smallest power of two that covers the
+// row: part of a warp (sums by shuffles; several rows per warp), or several warps (shuffles, then shared memory).
+// ================================================================================================
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
 
-// Sum over a block of kRowThreads threads, in a fixed order; every thread gets it. `part`: one value per warp.
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T* part) {
+template <typename T, int VEC, int N, int TEAM>
+struct Row {
+  static constexpr int E = VEC * N;
+  T v[E];
+  // elements beyond C are `fill`
+  __device__ __forceinline__ void load(const T* row, int C, int t, T fill) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();   // the previous sum has been read
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T s = T(0);
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TEAM + t) * VEC;
+      if (c < C) {
+        const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(row + c);
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) s += part[w];
-  return s;
+        for (int j = 0; j < VEC; ++j) v[i * VEC + j] = p.v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i * VEC + j] = fill;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int C, int t) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TEAM + t) * VEC;
+      if (c < C) {
+        Pack<T, VEC> p;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.v[j] = v[i * VEC + j];
+        *reinterpret_cast<Pack<T, VEC>*>(row + c) = p;
+      }
+    }
+  }
+};
+
+constexpr int kTeamThreads = 256;   // of a block, unless a team is larger
+template <int TEAM> constexpr int team_block() { return TEAM > kTeamThreads ? TEAM : kTeamThreads; }
+
+// Sums of K values over a team, in a fixed order; every thread gets them. `part`: the block's space for teams of several warps,
+// [2][warps][K]; consecutive calls alternate `turn`, so that one barrier separates a call's reads from the next but one's writes.
+template <int TEAM, int K, typename T>
+__device__ __forceinline__ void team_sums(T (&s)[K], T* part, int turn) {
+#pragma unroll
+  for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+  if (TEAM > 32) {
+    constexpr int kWarps = TEAM / 32, kAll = team_block<TEAM>() / 32;
+    const int warp = threadIdx.x >> 5, first = warp / kWarps * kWarps;
+    T* at = part + turn * kAll * K;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) at[warp * K + k] = s[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {   // lane w reads warp w's sum
+      const int lane = threadIdx.x & 31;
+      T t = lane < kWarps ? at[(first + lane) * K + k] : T(0);
+#pragma unroll
+      for (int o = (kWarps < 32 ? kWarps : 32) / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      s[k] = kWarps < 32 ? __shfl_sync(0xffffffffu, t, 0) : t;
+    }
+  }
 }
 
 __device__ __forceinline__ float inverse_root(float v) { return 1.0f / sqrtf(v); }
@@ -28,63 +85,197 @@ __device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v);
 
 // ================================================================================================
 // Layer norm: y = (x - m) / sqrt(v + eps) * gain + bias with the row's mean m and variance v (of the centred values, so
-// that a large common offset costs no digits).
+// that a large common offset costs no digits). Bound by the bytes of x and y: every row is read once, and the next row's loads
+// are under way while this row's sums are formed.
 // ================================================================================================
-template <typename T>
-__device__ __forceinline__ void row_statistics(const T* x, long C, T eps, T* part, T& mean, T& rstd) {
-  T s = T(0);
-  for (long c = threadIdx.x; c < C; c += kRowThreads) s += x[c];
-  mean = block_sum(s, part) / (T)C;
-  T q = T(0);
-  for (long c = threadIdx.x; c < C; c += kRowThreads) { const T d = x[c] - mean; q += d * d; }
-  rstd = inverse_root(block_sum(q, part) / (T)C + eps);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
-                                                                   long R, long C, T eps, T* __restrict__ y) {
-  __shared__ T part[kRowThreads / 32];
-  for (long r = blockIdx.x; r < R; r += gridDim.x) {
-    T mean, rstd;
-    row_statistics(x + r * C, C, eps, part, mean, rstd);
-    for (long c = threadIdx.x; c < C; c += kRowThreads) y[r * C + c] = (x[r * C + c] - mean) * rstd * gain[c] + bias[c];
+template <typename T, int VEC, int N, int TEAM>
+__global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
+                                                                          long R, int C, T eps, T* __restrict__ y) {
+  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  __shared__ T part[2 * (kBlock / 32) * 1];
+  const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+  Row<T, VEC, N, TEAM> g, b, row, next;
+  g.load(gain, C, t, T(0));
+  b.load(bias, C, t, T(0));
+  // all teams of a block make the same number of steps: they share barriers
+  const long step = (long)gridDim.x * kTeams;
+  long r = (long)blockIdx.x * kTeams + team;
+  if (r < R) next.load(x + r * C, C, t, T(0));
+  for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
+    row = next;
+    if (r + step < R) next.load(x + (r + step) * C, C, t, T(0));
+    T s[1] = {T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0] += row.v[e];
+    team_sums<TEAM>(s, part, 0);
+    const T mean = s[0] / (T)C;
+    T q[1] = {T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      row.v[e] -= mean;
+      if ((e / VEC * TEAM + t) * VEC + e % VEC < C) q[0] += row.v[e] * row.v[e];
+    }
+    team_sums<TEAM>(q, part, 1);
+    const T rstd = inverse_root(q[0] / (T)C + eps);
+    if (r < R) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) row.v[e] = row.v[e] * rstd * g.v[e] + b.v[e];
+      row.store(y + r * C, C, t);
+    }
   }
 }
 
-// dx = rstd * (d - mean(d) - xh * mean(d * xh)) with xh = (x - m) * rstd and d = gy * gain; the row's statistics are formed
-// again from x, which is read anyway, and kept for the sums over the rows.
+// Gradients, from one pass over x and gy: with d = gy * gain and xh = (x - m) * rstd
+//   dx = rstd * (d - mean(d) - xh * mean(d * xh)), dgain[c] = sum_r gy * xh, dbias[c] = sum_r gy.
+// The row's statistics are formed again from x, which is read anyway: two rounds of sums per row (x and d; the squares and the
+// products of the centred x). A thread sees the same columns in every row, so dgain and dbias are added up in registers; the
+// teams of a block join theirs through shared memory, the blocks through part[block][2][C], which norm_fold_kernel adds in order.
+template <typename T, int VEC, int N, int TEAM>
+__global__ void __launch_bounds__(team_block<TEAM>()) norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy,
+                                                                           long R, int C, T eps, T* __restrict__ dx, T* __restrict__ part) {
+  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  __shared__ T sums[2 * (kBlock / 32) * 2];
+  __shared__ T joined[kTeams > 1 ? 2 * E * kBlock : 1];
+  const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+  Row<T, VEC, N, TEAM> w, dg, db;
+  w.load(gain, C, t, T(0));
+#pragma unroll
+  for (int e = 0; e < E; ++e) dg.v[e] = db.v[e] = T(0);
+  const long step = (long)gridDim.x * kTeams;
+  long r = (long)blockIdx.x * kTeams + team;
+  for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
+    Row<T, VEC, N, TEAM> a, g;
+    const int valid = r < R ? C : 0;
+    a.load(x + r * C, valid, t, T(0));
+    g.load(gy + r * C, valid, t, T(0));
+    T s[2] = {T(0), T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s[0] += a.v[e];
+      s[1] += g.v[e] * w.v[e];
+    }
+    team_sums<TEAM>(s, sums, 0);
+    const T mean = s[0] / (T)C, s1 = s[1] / (T)C;
+    T q[2] = {T(0), T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      a.v[e] -= mean;
+      if ((e / VEC * TEAM + t) * VEC + e % VEC < C) q[0] += a.v[e] * a.v[e];
+      q[1] += g.v[e] * w.v[e] * a.v[e];      // g is 0 beyond C
+    }
+    team_sums<TEAM>(q, sums, 1);
+    const T rstd = inverse_root(q[0] / (T)C + eps), s2 = q[1] / (T)C * rstd;
+    if (r < R) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const T xh = a.v[e] * rstd;
+        dg.v[e] += g.v[e] * xh;
+        db.v[e] += g.v[e];
+        a.v[e] = rstd * (g.v[e] * w.v[e] - s1 - xh * s2);
+      }
+      a.store(dx + r * C, C, t);
+    }
+  }
+  T* out = part + (long)blockIdx.x * 2 * C;
+  if (kTeams == 1) {
+    dg.store(out, C, t);
+    db.store(out + C, C, t);
+  } else {
+    // [e][thread]; then thread j of the first team adds its columns over the teams, in order
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      joined[(2 * e) * kBlock + threadIdx.x] = dg.v[e];
+      joined[(2 * e + 1) * kBlock + threadIdx.x] = db.v[e];
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < 2 * E * TEAM; k += kBlock) {
+      const int j = k % TEAM, e = k / TEAM / 2, which = k / TEAM & 1;
+      T v = T(0);
+      for (int q = 0; q < kTeams; ++q) v += joined[(2 * e + which) * kBlock + q * TEAM + j];
+      const int c = (e / VEC * TEAM + j) * VEC + e % VEC;
+      if (c < C) out[(long)which * C + c] = v;
+    }
+  }
+}
+
+// dgain and dbias from the blocks' sums part[P][2][C]: 32 of the 2 C columns per block, 16 groups of threads that each add
+// every 16th block's, then the groups in order
+constexpr int kFoldGroups = 16;
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy,
-                                                                    long R, long C, T eps, T* __restrict__ dx, T* __restrict__ stats) {
-  __shared__ T part[kRowThreads / 32];
+__global__ void __launch_bounds__(32 * kFoldGroups) norm_fold_kernel(const T* __restrict__ part, long C, int P, T* __restrict__ dgain, T* __restrict__ dbias) {
+  __shared__ T joined[kFoldGroups][32];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const long c = (long)blockIdx.x * 32 + lane;
+  T s = T(0);
+  if (c < 2 * C) {
+#pragma unroll 8
+    for (int q = group; q < P; q += kFoldGroups) s += part[(long)q * 2 * C + c];
+  }
+  joined[group][lane] = s;
+  __syncthreads();
+  if (group == 0 && c < 2 * C) {
+#pragma unroll
+    for (int q = 1; q < kFoldGroups; ++q) s += joined[q][lane];
+    if (c < C) dgain[c] = s;
+    else dbias[c - C] = s;
+  }
+}
+
+// ---- rows that no team holds: a block per row that reads it several times (the L2 cache has it) ----
+constexpr int kLongThreads = 1024;
+template <typename T>
+__device__ __forceinline__ void long_row_statistics(const T* x, long C, T eps, T* part, T& mean, T& rstd) {
+  T s[1] = {T(0)};
+  for (long c = threadIdx.x; c < C; c += kLongThreads) s[0] += x[c];
+  team_sums<kLongThreads>(s, part, 0);
+  mean = s[0] / (T)C;
+  T q[1] = {T(0)};
+  for (long c = threadIdx.x; c < C; c += kLongThreads) { const T d = x[c] - mean; q[0] += d * d; }
+  team_sums<kLongThreads>(q, part, 1);
+  rstd = inverse_root(q[0] / (T)C + eps);
+}
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) norm_forward_long_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
+                                                                         long R, long C, T eps, T* __restrict__ y) {
+  __shared__ T part[2 * 32];
   for (long r = blockIdx.x; r < R; r += gridDim.x) {
     T mean, rstd;
-    row_statistics(x + r * C, C, eps, part, mean, rstd);
-    T s1 = T(0), s2 = T(0);
-    for (long c = threadIdx.x; c < C; c += kRowThreads) {
+    long_row_statistics(x + r * C, C, eps, part, mean, rstd);
+    for (long c = threadIdx.x; c < C; c += kLongThreads) y[r * C + c] = (x[r * C + c] - mean) * rstd * gain[c] + bias[c];
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy,
+                                                                          long R, long C, T eps, T* __restrict__ dx, T* __restrict__ stats) {
+  __shared__ T part[2 * 32 + 32 * 2];
+  for (long r = blockIdx.x; r < R; r += gridDim.x) {
+    T mean, rstd;
+    long_row_statistics(x + r * C, C, eps, part, mean, rstd);
+    T s[2] = {T(0), T(0)};
+    for (long c = threadIdx.x; c < C; c += kLongThreads) {
       const T d = gy[r * C + c] * gain[c];
-      s1 += d;
-      s2 += d * ((x[r * C + c] - mean) * rstd);
+      s[0] += d;
+      s[1] += d * ((x[r * C + c] - mean) * rstd);
     }
-    s1 = block_sum(s1, part) / (T)C;
-    s2 = block_sum(s2, part) / (T)C;
-    for (long c = threadIdx.x; c < C; c += kRowThreads) {
+    team_sums<kLongThreads>(s, part + 2 * 32, 0);
+    const T s1 = s[0] / (T)C, s2 = s[1] / (T)C;
+    for (long c = threadIdx.x; c < C; c += kLongThreads) {
       const T d = gy[r * C + c] * gain[c], xh = (x[r * C + c] - mean) * rstd;
       dx[r * C + c] = rstd * (d - s1 - xh * s2);
     }
     if (threadIdx.x == 0) { stats[2 * r] = mean; stats[2 * r + 1] = rstd; }
   }
 }
-
 // sums over the rows of slice blockIdx.y: part[slice][0][c] of gy * xh, part[slice][1][c] of gy
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_columns_kernel(const T* __restrict__ x, const T* __restrict__ gy, const T* __restrict__ stats,
-                                                                   long R, long C, long rows_per_slice, T* __restrict__ part) {
-  const long c = (long)blockIdx.x * kRowThreads + threadIdx.x;
+__global__ void __launch_bounds__(256) norm_columns_kernel(const T* __restrict__ x, const T* __restrict__ gy, const T* __restrict__ stats,
+                                                           long R, long C, long rows_per_slice, T* __restrict__ part) {
+  const long c = (long)blockIdx.x * 256 + threadIdx.x;
   if (c >= C) return;
   const long first = blockIdx.y * rows_per_slice;
   const long last = first + rows_per_slice < R ? first + rows_per_slice : R;
   T s1 = T(0), s2 = T(0);
+#pragma unroll 4
   for (long r = first; r < last; ++r) {
     const T g = gy[r * C + c];
     s1 += g * ((x[r * C + c] - stats[2 * r]) * stats[2 * r + 1]);
@@ -94,39 +285,93 @@ __global__ void __launch_bounds__(kRowThreads) norm_columns_kernel(const T* __re
   part[(2 * (long)blockIdx.y + 1) * C + c] = s2;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_fold_kernel(const T* __restrict__ part, long C, int slices, T* __restrict__ dgain, T* __restrict__ dbias) {
-  const long c = (long)blockIdx.x * kRowThreads + threadIdx.x;
-  if (c >= C) return;
-  T s1 = T(0), s2 = T(0);
-  for (int s = 0; s < slices; ++s) {
-    s1 += part[(2L * s) * C + c];
-    s2 += part[(2L * s + 1) * C + c];
-  }
-  dgain[c] = s1;
-  dbias[c] = s2;
+template <typename T> bool starts_on_16(long C, std::initializer_list<const void*> arrays) {
+  if (C * sizeof(T) % 16) return false;
+  for (const void* a : arrays)
+    if ((uintptr_t)a & 15) return false;
+  return true;
+}
+
+// calls f(vec, team) with the team's constants for rows of C elements, E of them a thread; false when no team is large enough
+template <int E, int kMaxTeam, typename F>
+bool with_team(long C, F f) {
+  if (C <= 1L * E) f(std::integral_constant<int, 1>());
+  else if (C <= 2L * E) f(std::integral_constant<int, 2>());
+  else if (C <= 4L * E) f(std::integral_constant<int, 4>());
+  else if (C <= 8L * E) f(std::integral_constant<int, 8>());
+  else if (C <= 16L * E) f(std::integral_constant<int, 16>());
+  else if (C <= 32L * E) f(std::integral_constant<int, 32>());
+  else if (C <= 64L * E) f(std::integral_constant<int, 64>());
+  else if (C <= 128L * E) f(std::integral_constant<int, 128>());
+  else if (C <= 256L * E) f(std::integral_constant<int, 256>());
+  else if (C <= 512L * E) f(std::integral_constant<int, 512>());
+  else if (C <= 1024L * E) f(std::integral_constant<int, 1024>());
+  else return false;
+  return true;
+}
+
+// as many blocks as the SMs hold at a time: the grid of a kernel whose blocks walk the rows
+template <typename K>
+unsigned resident_blocks(K kernel, int threads) {
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+  return (unsigned)(rt().sm_count * per_sm);
 }
 
 template <typename T>
 int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, double eps, T* y) {
-  const long grid = R < 65536 ? R : 65536;
-  CGTB_LAUNCH(norm_forward_kernel<T>, (unsigned)grid, kRowThreads, 0, x, gain, bias, R, C, (T)eps, y);
+  constexpr int E = 32 / sizeof(T);     // 8 float32 or 4 float64 a thread
+  const bool wide = starts_on_16<T>(C, {x, gain, bias, y});
+  const bool held = with_team<E, 1024>(C, [&](auto team) {
+    constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
+    auto launch = [&](auto kernel) {
+      static const unsigned most = resident_blocks(kernel, kBlock);
+      const long blocks = cgtb_ceil_div(R, kBlock / TEAM);
+      CGTB_LAUNCH(kernel, (unsigned)(blocks < most ? blocks : most), kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y);
+    };
+    if (wide) launch(norm_forward_kernel<T, 16 / sizeof(T), 2, TEAM>);
+    else launch(norm_forward_kernel<T, 1, E, TEAM>);
+  });
+  if (!held) {
+    const long grid = R < rt().sm_count * 2L ? R : rt().sm_count * 2L;
+    CGTB_LAUNCH(norm_forward_long_kernel<T>, (unsigned)grid, kLongThreads, 0, x, gain, bias, R, C, (T)eps, y);
+  }
   CGTB_CHECK_LAUNCH("layer_norm_forward");
   return 0;
 }
 
 template <typename T>
 int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias) {
-  const long cblocks = cgtb_ceil_div(C, kRowThreads);
-  long slices = cgtb_ceil_div(R, 64);
-  if (slices > 64) slices = 64;
-  T* stats = (T*)scratch((size_t)(2 * R + 2 * slices * C) * sizeof(T));
-  if (!stats) return 1;
-  T* part = stats + 2 * R;
-  const long grid = R < 65536 ? R : 65536;
-  CGTB_LAUNCH(norm_backward_kernel<T>, (unsigned)grid, kRowThreads, 0, x, gain, gy, R, C, (T)eps, dx, stats);
-  CGTB_LAUNCH(norm_columns_kernel<T>, dim3((unsigned)cblocks, (unsigned)slices), kRowThreads, 0, x, gy, stats, R, C, cgtb_ceil_div(R, slices), part);
-  CGTB_LAUNCH(norm_fold_kernel<T>, (unsigned)cblocks, kRowThreads, 0, part, C, (int)slices, dgain, dbias);
+  constexpr int E = 32 / sizeof(T);
+  const bool wide = starts_on_16<T>(C, {x, gain, gy, dx});
+  T* part = nullptr;
+  long P = 0;
+  const bool held = with_team<E, 1024>(C, [&](auto team) {
+    constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
+    auto launch = [&](auto kernel) {
+      static const unsigned most = resident_blocks(kernel, kBlock);
+      // at least eight rows for a team: what the blocks leave for the last kernel stays small against the rows
+      const long blocks = cgtb_ceil_div(cgtb_ceil_div(R, 8), kTeams);
+      P = blocks < most ? blocks : most;
+      part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
+      if (part) CGTB_LAUNCH(kernel, (unsigned)P, kBlock, 0, x, gain, gy, R, (int)C, (T)eps, dx, part);
+    };
+    if (wide) launch(norm_backward_kernel<T, 16 / sizeof(T), 2, TEAM>);
+    else launch(norm_backward_kernel<T, 1, E, TEAM>);
+  });
+  if (!held) {
+    const long cblocks = cgtb_ceil_div(C, 256);
+    P = cgtb_ceil_div(R, 64);
+    if (P > 64) P = 64;
+    T* stats = (T*)scratch((size_t)(2 * R + 2 * P * C) * sizeof(T));
+    if (!stats) return 1;
+    part = stats + 2 * R;
+    const long grid = R < rt().sm_count * 2L ? R : rt().sm_count * 2L;
+    CGTB_LAUNCH(norm_backward_long_kernel<T>, (unsigned)grid, kLongThreads, 0, x, gain, gy, R, C, (T)eps, dx, stats);
+    CGTB_LAUNCH(norm_columns_kernel<T>, dim3((unsigned)cblocks, (unsigned)P), 256, 0, x, gy, stats, R, C, cgtb_ceil_div(R, P), part);
+  }
+  if (!part) return 1;
+  CGTB_LAUNCH(norm_fold_kernel<T>, (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
   CGTB_CHECK_LAUNCH("layer_norm_backward");
   return 0;
 }
@@ -182,20 +427,21 @@ __device__ __forceinline__ float code_of(float x, float largest, float inverse) 
   return fabsf(t - k) < 0.4999f ? k : code_exact(x, largest);   // also for an inverse that overflows: then t is not finite
 }
 
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const float* __restrict__ x, long R, long C, long Cp, int8_t* __restrict__ codes,
+constexpr int kQuantThreads = 256;
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const float* __restrict__ x, long R, long C, long Cp, int8_t* __restrict__ codes,
                                                                     float* __restrict__ scales) {
-  __shared__ uint32_t part[kRowThreads / 32];
+  __shared__ uint32_t part[kQuantThreads / 32];
   for (long r = blockIdx.x; r < R; r += gridDim.x) {
     uint32_t m = 0;   // as whole numbers the bits of |x| order like the values, infinities and NaN above all
-    for (long c = threadIdx.x; c < C; c += kRowThreads) m = max(m, __float_as_uint(x[r * C + c]) & 0x7fffffffu);
+    for (long c = threadIdx.x; c < C; c += kQuantThreads) m = max(m, __float_as_uint(x[r * C + c]) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
-    for (int w = 0; w < kRowThreads / 32; ++w) m = max(m, part[w]);
+    for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, part[w]);
     const bool finite = m < 0x7f800000u;
     const float largest = __uint_as_float(m), inverse = 127.0f / largest;
-    for (long c = threadIdx.x; c < Cp; c += kRowThreads)
+    for (long c = threadIdx.x; c < Cp; c += kQuantThreads)
       codes[r * Cp + c] = (int8_t)(c < C && finite && m != 0 ? code_of(x[r * C + c], largest, inverse) : 0.0f);
     if (threadIdx.x == 0) scales[r] = finite ? largest / 127.0f : __uint_as_float(0x7fc00000u);
   }
@@ -252,7 +498,7 @@ CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, f
   if (R < 0 || C < 0) return fail("cgtb_quantize_rows: negative extent");
   if (R == 0) return 0;
   const unsigned grid = (unsigned)(R < 65536 ? R : 65536);
-  CGTB_LAUNCH(quantize_rows_kernel, grid, kRowThreads, 0, x, R, C, cgtb_ceil_div(C, 16) * 16, codes, scales);
+  CGTB_LAUNCH(quantize_rows_kernel, grid, kQuantThreads, 0, x, R, C, cgtb_ceil_div(C, 16) * 16, codes, scales);
   CGTB_CHECK_LAUNCH("quantize_rows");
   return 0;
 }
