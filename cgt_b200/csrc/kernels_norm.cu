@@ -1,6 +1,7 @@
 // Layer norm with its gradients, dropout from a counter-based generator, and rows in 8-bit integers with a scale each, for
 // sm_100a.
 #include "runtime.h"
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -125,29 +126,72 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
   }
 }
 
+// One element group of a thread from global to shared memory, asynchronously
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+
 // Gradients, from one pass over x and gy: with d = gy * gain and xh = (x - m) * rstd
 //   dx = rstd * (d - mean(d) - xh * mean(d * xh)), dgain[c] = sum_r gy * xh, dbias[c] = sum_r gy.
 // The row's statistics are formed again from x, which is read anyway: two rounds of sums per row (x and d; the squares and the
 // products of the centred x). A thread sees the same columns in every row, so dgain and dbias are added up in registers; the
 // teams of a block join theirs through shared memory, the blocks through part[block][2][C], which norm_fold_kernel adds in order.
+// Bound by the bytes of x, gy and dx. What a thread will need of the next kAhead rows is on its way into its own places of shared
+// memory (no other thread touches them: no barrier): registers could hold one row more at most.
+constexpr int kAhead = 2;
 template <typename T, int VEC, int N, int TEAM>
-__global__ void __launch_bounds__(team_block<TEAM>()) norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy,
-                                                                           long R, int C, T eps, T* __restrict__ dx, T* __restrict__ part) {
+constexpr size_t norm_backward_bytes() { return (size_t)(kAhead + 1) * 2 * N * team_block<TEAM>() * VEC * sizeof(T); }
+
+template <typename T, int VEC, int N, int TEAM>
+__global__ void __launch_bounds__(team_block<TEAM>(), (sizeof(T) == 4 || TEAM == 1024 ? 1024 : 512) / team_block<TEAM>())
+norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy, long R, int C, T eps, T* __restrict__ dx,
+                     T* __restrict__ part) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  typedef Pack<T, VEC> P;
+  extern __shared__ __align__(16) unsigned char ahead_raw[];
   __shared__ T sums[2 * (kBlock / 32) * 2];
-  __shared__ T joined[kTeams > 1 ? 2 * E * kBlock : 1];
+  P* ahead = reinterpret_cast<P*>(ahead_raw) + threadIdx.x;     // [kAhead + 1][x, gy][N][thread]
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+  const long step = (long)gridDim.x * kTeams;
+  auto fetch = [&](int stage, long r) {
+    if (r < R) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * TEAM + t) * VEC;
+        if (c < C) {
+          copy_async<sizeof(P)>(ahead + (stage * 2 * N + i) * kBlock, x + r * C + c);
+          copy_async<sizeof(P)>(ahead + (stage * 2 * N + N + i) * kBlock, gy + r * C + c);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  long r = (long)blockIdx.x * kTeams + team;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) fetch(i, r + i * step);
   Row<T, VEC, N, TEAM> w, dg, db;
   w.load(gain, C, t, T(0));
 #pragma unroll
   for (int e = 0; e < E; ++e) dg.v[e] = db.v[e] = T(0);
-  const long step = (long)gridDim.x * kTeams;
-  long r = (long)blockIdx.x * kTeams + team;
+  int stage = 0;
   for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
+    fetch(stage >= 1 ? stage - 1 : kAhead, r + kAhead * step);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
     Row<T, VEC, N, TEAM> a, g;
-    const int valid = r < R ? C : 0;
-    a.load(x + r * C, valid, t, T(0));
-    g.load(gy + r * C, valid, t, T(0));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool valid = r < R && (i * TEAM + t) * VEC < C;
+      const P px = ahead[(stage * 2 * N + i) * kBlock], pg = ahead[(stage * 2 * N + N + i) * kBlock];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        a.v[i * VEC + j] = valid ? px.v[j] : T(0);
+        g.v[i * VEC + j] = valid ? pg.v[j] : T(0);
+      }
+    }
+    if (++stage > kAhead) stage = 0;
     T s[2] = {T(0), T(0)};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -177,11 +221,14 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_backward_kernel(const
     }
   }
   T* out = part + (long)blockIdx.x * 2 * C;
+  T* joined = reinterpret_cast<T*>(ahead_raw);      // 2 E of the block's threads: less than the rows took
   if (kTeams == 1) {
     dg.store(out, C, t);
     db.store(out + C, C, t);
   } else {
-    // [e][thread]; then thread j of the first team adds its columns over the teams, in order
+    // [e][thread]; then the columns are added over the teams, in order
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       joined[(2 * e) * kBlock + threadIdx.x] = dg.v[e];
@@ -311,11 +358,15 @@ bool with_team(long C, F f) {
 }
 
 // as many blocks as the SMs hold at a time: the grid of a kernel whose blocks walk the rows
-template <typename K>
-unsigned resident_blocks(K kernel, int threads) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
-  return (unsigned)(rt().sm_count * per_sm);
+template <auto KERNEL, int THREADS, size_t BYTES>
+long resident_blocks() {
+  static const long n = [] {
+    int per_sm = 0;
+    if (BYTES > 32 * 1024) cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES);   // with static memory: over 48 KB
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, THREADS, BYTES) != cudaSuccess || per_sm < 1) per_sm = 1;
+    return (long)rt().sm_count * per_sm;
+  }();
+  return n;
 }
 
 template <typename T>
@@ -324,13 +375,13 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   const bool wide = starts_on_16<T>(C, {x, gain, bias, y});
   const bool held = with_team<E, 1024>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
-    auto launch = [&](auto kernel) {
-      static const unsigned most = resident_blocks(kernel, kBlock);
-      const long blocks = cgtb_ceil_div(R, kBlock / TEAM);
-      CGTB_LAUNCH(kernel, (unsigned)(blocks < most ? blocks : most), kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y);
+    auto launch = [&](auto width) {
+      constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, E / decltype(width)::value, TEAM>;
+      const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
+      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y);
     };
-    if (wide) launch(norm_forward_kernel<T, 16 / sizeof(T), 2, TEAM>);
-    else launch(norm_forward_kernel<T, 1, E, TEAM>);
+    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
+    else launch(std::integral_constant<int, 1>());
   });
   if (!held) {
     const long grid = R < rt().sm_count * 2L ? R : rt().sm_count * 2L;
@@ -348,16 +399,19 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   long P = 0;
   const bool held = with_team<E, 1024>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
-    auto launch = [&](auto kernel) {
-      static const unsigned most = resident_blocks(kernel, kBlock);
-      // at least eight rows for a team: what the blocks leave for the last kernel stays small against the rows
-      const long blocks = cgtb_ceil_div(cgtb_ceil_div(R, 8), kTeams);
-      P = blocks < most ? blocks : most;
+    auto launch = [&](auto width) {
+      constexpr int VEC = decltype(width)::value;
+      constexpr size_t bytes = norm_backward_bytes<T, VEC, E / VEC, TEAM>();
+      constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM>;
+      // at least four rows for a team, so that what the blocks leave for the last kernel stays small against the rows; but no SM
+      // without a block where there are rows for it
+      const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
+      P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
       part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
-      if (part) CGTB_LAUNCH(kernel, (unsigned)P, kBlock, 0, x, gain, gy, R, (int)C, (T)eps, dx, part);
+      if (part) CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part);
     };
-    if (wide) launch(norm_backward_kernel<T, 16 / sizeof(T), 2, TEAM>);
-    else launch(norm_backward_kernel<T, 1, E, TEAM>);
+    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
+    else launch(std::integral_constant<int, 1>());
   });
   if (!held) {
     const long cblocks = cgtb_ceil_div(C, 256);
