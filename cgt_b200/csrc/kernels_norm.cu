@@ -54,29 +54,47 @@ struct Row {
 constexpr int kTeamThreads = 256;   // of a block, unless a team is larger
 template <int TEAM> constexpr int team_block() { return TEAM > kTeamThreads ? TEAM : kTeamThreads; }
 
-// Sums of K values over a team, in a fixed order; every thread gets them. `part`: the block's space for teams of several warps,
-// [2][warps][K]; consecutive calls alternate `turn`, so that one barrier separates a call's reads from the next but one's writes.
+// Sums of one or two values over a team, in a fixed order; every thread gets them. `part`: the block's space for teams of several
+// warps, 2 * K * (warps of the block) values; consecutive calls alternate `turn`, so that one barrier separates a call's reads
+// from the next but one's writes. Two values cost little more than one: after the first step half of the lanes go on with
+// either of them.
 template <int TEAM, int K, typename T>
 __device__ __forceinline__ void team_sums(T (&s)[K], T* part, int turn) {
+  constexpr int kLanes = TEAM < 32 ? TEAM : 32, kWarps = TEAM / 32, kAll = team_block<TEAM>() / 32;
+  const int lane = threadIdx.x & 31;
+  T v = s[0];
+  if constexpr (K == 2 && kLanes > 1) {
+    const bool upper = lane & (kLanes / 2);
+    v = (upper ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, upper ? s[0] : s[1], kLanes / 2);
+  }
 #pragma unroll
-  for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-  if (TEAM > 32) {
-    constexpr int kWarps = TEAM / 32, kAll = team_block<TEAM>() / 32;
+  for (int o = kLanes / (2 * K); o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TEAM <= 32) {
+    if constexpr (K == 1) s[0] = v;
+    else if constexpr (kLanes > 1) {
+      const T other = __shfl_xor_sync(0xffffffffu, v, kLanes / 2);
+      const bool upper = lane & (kLanes / 2);
+      s[0] = upper ? other : v;
+      s[1] = upper ? v : other;
+    }
+  } else {
     const int warp = threadIdx.x >> 5, first = warp / kWarps * kWarps;
-    T* at = part + turn * kAll * K;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int k = 0; k < K; ++k) at[warp * K + k] = s[k];
+    T* at = part + turn * kAll * K;           // [K][warp]
+    if ((lane & 15) == 0 && (K == 2 || lane == 0)) at[(lane >> 4) * kAll + warp] = v;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {   // lane w reads warp w's sum
-      const int lane = threadIdx.x & 31;
-      T t = lane < kWarps ? at[(first + lane) * K + k] : T(0);
+    for (int k = 0; k < K; ++k) {
+      T t;
+      if constexpr (kWarps <= 8) {            // every thread adds them
+        t = at[k * kAll + first];
 #pragma unroll
-      for (int o = (kWarps < 32 ? kWarps : 32) / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      s[k] = kWarps < 32 ? __shfl_sync(0xffffffffu, t, 0) : t;
+        for (int w = 1; w < kWarps; ++w) t += at[k * kAll + first + w];
+      } else {                                // lane w takes warp w's
+        t = at[k * kAll + first + (lane & (kWarps - 1))];
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      }
+      s[k] = t;
     }
   }
 }
@@ -96,6 +114,9 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
   __shared__ T part[2 * (kBlock / 32) * 1];
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   Row<T, VEC, N, TEAM> g, b, row, next;
+  bool inside[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) inside[i] = (i * TEAM + t) * VEC < C;
   g.load(gain, C, t, T(0));
   b.load(bias, C, t, T(0));
   // all teams of a block make the same number of steps: they share barriers
@@ -114,7 +135,7 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       row.v[e] -= mean;
-      if ((e / VEC * TEAM + t) * VEC + e % VEC < C) q[0] += row.v[e] * row.v[e];
+      q[0] += inside[e / VEC] ? row.v[e] * row.v[e] : T(0);
     }
     team_sums<TEAM>(q, part, 1);
     const T rstd = inverse_root(q[0] / (T)C + eps);
@@ -146,26 +167,34 @@ template <typename T, int VEC, int N, int TEAM>
 constexpr size_t norm_backward_bytes() { return (size_t)(kAhead + 1) * 2 * N * team_block<TEAM>() * VEC * sizeof(T); }
 
 template <typename T, int VEC, int N, int TEAM>
-__global__ void __launch_bounds__(team_block<TEAM>(), (sizeof(T) == 4 || TEAM == 1024 ? 1024 : 512) / team_block<TEAM>())
+__global__ void __launch_bounds__(team_block<TEAM>(), (TEAM == 1024 || VEC * N * sizeof(T) == 32 && sizeof(T) == 4 ? 1024 : 512) / team_block<TEAM>())
 norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy, long R, int C, T eps, T* __restrict__ dx,
                      T* __restrict__ part) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
   typedef Pack<T, VEC> P;
   extern __shared__ __align__(16) unsigned char ahead_raw[];
-  __shared__ T sums[2 * (kBlock / 32) * 2];
+  __shared__ __align__(16) T sums[2 * (kBlock / 32) * 2];
   P* ahead = reinterpret_cast<P*>(ahead_raw) + threadIdx.x;     // [kAhead + 1][x, gy][N][thread]
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   const long step = (long)gridDim.x * kTeams;
+  bool inside[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    inside[i] = (i * TEAM + t) * VEC < C;
+    if (!inside[i])      // never written again: columns beyond C are zeros in every row
+      for (int k = 0; k < 2 * (kAhead + 1); ++k)
+        for (int j = 0; j < VEC; ++j) ahead[(k * N + i) * kBlock].v[j] = T(0);
+  }
   auto fetch = [&](int stage, long r) {
     if (r < R) {
+      const T *from_x = x + r * C + t * VEC, *from_g = gy + r * C + t * VEC;
+      P* to = ahead + stage * (2 * N * kBlock);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = (i * TEAM + t) * VEC;
-        if (c < C) {
-          copy_async<sizeof(P)>(ahead + (stage * 2 * N + i) * kBlock, x + r * C + c);
-          copy_async<sizeof(P)>(ahead + (stage * 2 * N + N + i) * kBlock, gy + r * C + c);
+      for (int i = 0; i < N; ++i)
+        if (inside[i]) {
+          copy_async<sizeof(P)>(to + i * kBlock, from_x + i * TEAM * VEC);
+          copy_async<sizeof(P)>(to + (N + i) * kBlock, from_g + i * TEAM * VEC);
         }
-      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -181,14 +210,14 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
     fetch(stage >= 1 ? stage - 1 : kAhead, r + kAhead * step);
     asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
     Row<T, VEC, N, TEAM> a, g;
+    const P* from = ahead + stage * (2 * N * kBlock);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool valid = r < R && (i * TEAM + t) * VEC < C;
-      const P px = ahead[(stage * 2 * N + i) * kBlock], pg = ahead[(stage * 2 * N + N + i) * kBlock];
+      const P px = from[i * kBlock], pg = from[(N + i) * kBlock];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        a.v[i * VEC + j] = valid ? px.v[j] : T(0);
-        g.v[i * VEC + j] = valid ? pg.v[j] : T(0);
+        a.v[i * VEC + j] = px.v[j];
+        g.v[i * VEC + j] = pg.v[j];
       }
     }
     if (++stage > kAhead) stage = 0;
@@ -204,7 +233,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       a.v[e] -= mean;
-      if ((e / VEC * TEAM + t) * VEC + e % VEC < C) q[0] += a.v[e] * a.v[e];
+      q[0] += inside[e / VEC] ? a.v[e] * a.v[e] : T(0);
       q[1] += g.v[e] * w.v[e] * a.v[e];      // g is 0 beyond C
     }
     team_sums<TEAM>(q, sums, 1);
@@ -245,9 +274,9 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
   }
 }
 
-// dgain and dbias from the blocks' sums part[P][2][C]: 32 of the 2 C columns per block, 16 groups of threads that each add
-// every 16th block's, then the groups in order
-constexpr int kFoldGroups = 16;
+// dgain and dbias from the blocks' sums part[P][2][C]: 32 of the 2 C columns per block, 32 groups of threads that each add
+// every 32nd block's, then the groups in order
+constexpr int kFoldGroups = 32;
 template <typename T>
 __global__ void __launch_bounds__(32 * kFoldGroups) norm_fold_kernel(const T* __restrict__ part, long C, int P, T* __restrict__ dgain, T* __restrict__ dbias) {
   __shared__ T joined[kFoldGroups][32];
@@ -339,7 +368,7 @@ template <typename T> bool starts_on_16(long C, std::initializer_list<const void
   return true;
 }
 
-// calls f(vec, team) with the team's constants for rows of C elements, E of them a thread; false when no team is large enough
+// calls f(team) with the smallest team for rows of C elements, E of them a thread; false when none is large enough
 template <int E, int kMaxTeam, typename F>
 bool with_team(long C, F f) {
   if (C <= 1L * E) f(std::integral_constant<int, 1>());
@@ -350,10 +379,12 @@ bool with_team(long C, F f) {
   else if (C <= 32L * E) f(std::integral_constant<int, 32>());
   else if (C <= 64L * E) f(std::integral_constant<int, 64>());
   else if (C <= 128L * E) f(std::integral_constant<int, 128>());
-  else if (C <= 256L * E) f(std::integral_constant<int, 256>());
-  else if (C <= 512L * E) f(std::integral_constant<int, 512>());
-  else if (C <= 1024L * E) f(std::integral_constant<int, 1024>());
-  else return false;
+  else if constexpr (kMaxTeam >= 1024) {
+    if (C <= 256L * E) f(std::integral_constant<int, 256>());
+    else if (C <= 512L * E) f(std::integral_constant<int, 512>());
+    else if (C <= 1024L * E) f(std::integral_constant<int, 1024>());
+    else return false;
+  } else return false;
   return true;
 }
 
@@ -391,13 +422,11 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   return 0;
 }
 
-template <typename T>
-int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias) {
-  constexpr int E = 32 / sizeof(T);
+// The gradients by teams of E elements a thread: the rows' sums in `part` for P blocks. 1: failed, -1: no team is that large
+template <typename T, int E, int kMaxTeam>
+int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T*& part, long& P) {
   const bool wide = starts_on_16<T>(C, {x, gain, gy, dx});
-  T* part = nullptr;
-  long P = 0;
-  const bool held = with_team<E, 1024>(C, [&](auto team) {
+  const bool held = with_team<E, kMaxTeam>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
     auto launch = [&](auto width) {
       constexpr int VEC = decltype(width)::value;
@@ -413,7 +442,21 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
     else launch(std::integral_constant<int, 1>());
   });
-  if (!held) {
+  return !held ? -1 : part ? 0 : 1;
+}
+
+template <typename T>
+int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias) {
+  T* part = nullptr;
+  long P = 0;
+  // 16 elements a thread save steps of the sums (float32, 30000 x 784: 72 us with 8, 48 us with 16); with teams of more than four
+  // warps too few rows are under way at a time (8192 x 4096: 79 us with 8, 85 us with 16), with float64 registers run out
+  // (8192 x 1024: 46 us with 4, 51 us with 8)
+  int failed;
+  if (sizeof(T) == 4 && C > 16 && C <= 2048) failed = norm_backward_teams<T, 16, 128>(x, gain, gy, R, C, eps, dx, part, P);
+  else failed = norm_backward_teams<T, 32 / sizeof(T), 1024>(x, gain, gy, R, C, eps, dx, part, P);
+  if (failed > 0) return 1;
+  if (failed < 0) {
     const long cblocks = cgtb_ceil_div(C, 256);
     P = cgtb_ceil_div(R, 64);
     if (P > 64) P = 64;
@@ -424,7 +467,6 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     CGTB_LAUNCH(norm_backward_long_kernel<T>, (unsigned)grid, kLongThreads, 0, x, gain, gy, R, C, (T)eps, dx, stats);
     CGTB_LAUNCH(norm_columns_kernel<T>, dim3((unsigned)cblocks, (unsigned)P), 256, 0, x, gy, stats, R, C, cgtb_ceil_div(R, P), part);
   }
-  if (!part) return 1;
   CGTB_LAUNCH(norm_fold_kernel<T>, (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
   CGTB_CHECK_LAUNCH("layer_norm_backward");
   return 0;
