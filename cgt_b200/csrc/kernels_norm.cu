@@ -495,18 +495,58 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
   return c;
 }
 
-template <typename T>
+// A thread makes UNROLL blocks of four words, their elements loaded beforehand, 16 bytes at a time where the arrays start on
+// 16-byte boundaries. Bound by the bytes of x and y; the ten rounds of a block are forty multiplications for four elements.
+template <typename T, bool WIDE, int UNROLL>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, long n, uint32_t threshold, T scale, const long* __restrict__ state,
                                                       uint32_t site, T* y) {
-  const unsigned long long seed = (unsigned long long)state[0], step = (unsigned long long)state[1];
-  const long blocks = (n + 3) / 4;
-  for (long b = blockIdx.x * 256L + threadIdx.x; b < blocks; b += gridDim.x * 256L) {
-    const uint4 w = philox(make_uint4((uint32_t)b, (uint32_t)((unsigned long long)b >> 32), (uint32_t)step, site), make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  constexpr int kPack = WIDE ? 16 / sizeof(T) : 1, kPacks = 4 / kPack;
+  typedef Pack<T, kPack> P;
+  const unsigned long long seed = (unsigned long long)state[0];
+  const uint32_t step = (uint32_t)(unsigned long long)state[1];
+  const uint2 key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
+  const long whole = n / 4, stride = (long)gridDim.x * 256;
+  long b = (long)blockIdx.x * 256 + threadIdx.x;
+  for (; b < whole; b += UNROLL * stride) {
+    P v[UNROLL][kPacks];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * b + j < n) y[4 * b + j] = ws[j] >= threshold ? x[4 * b + j] * scale : T(0);
+    for (int u = 0; u < UNROLL; ++u)
+      if (b + u * stride < whole)
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) v[u][i] = reinterpret_cast<const P*>(x + 4 * (b + u * stride))[i];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const unsigned long long at = (unsigned long long)(b + u * stride);
+      if (b + u * stride < whole) {
+        const uint4 w = philox(make_uint4((uint32_t)at, (uint32_t)(at >> 32), step, site), key);
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) {
+#pragma unroll
+          for (int j = 0; j < kPack; ++j) v[u][i].v[j] = words[i * kPack + j] >= threshold ? v[u][i].v[j] * scale : T(0);
+          reinterpret_cast<P*>(y + 4 * at)[i] = v[u][i];
+        }
+      }
+    }
   }
+  // the last block's one to three elements
+  if (blockIdx.x == 0 && threadIdx.x < n % 4) {
+    const uint4 w = philox(make_uint4((uint32_t)whole, (uint32_t)((unsigned long long)whole >> 32), step, site), key);
+    const uint32_t mine = threadIdx.x == 0 ? w.x : threadIdx.x == 1 ? w.y : w.z;
+    const long i = 4 * whole + threadIdx.x;
+    y[i] = mine >= threshold ? x[i] * scale : T(0);
+  }
+}
+
+template <typename T>
+void dropout(const T* x, long n, uint32_t threshold, double scale, const int64_t* state, unsigned site, T* y) {
+  const bool wide = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
+  const long blocks = cgtb_ceil_div(cgtb_ceil_div(n, 4), 256);
+  auto launch = [&](auto kernel) {
+    CGTB_LAUNCH(kernel, (unsigned)std::min<long>(blocks, rt().sm_count * 8L), 256, 0, x, n, threshold, (T)scale, (const long*)state, site, y);
+  };
+  if (wide) launch(dropout_kernel<T, true, 2>);
+  else launch(dropout_kernel<T, false, 2>);
 }
 
 // ================================================================================================
@@ -523,23 +563,80 @@ __device__ __forceinline__ float code_of(float x, float largest, float inverse) 
   return fabsf(t - k) < 0.4999f ? k : code_exact(x, largest);   // also for an inverse that overflows: then t is not finite
 }
 
-constexpr int kQuantThreads = 256;
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const float* __restrict__ x, long R, long C, long Cp, int8_t* __restrict__ codes,
-                                                                    float* __restrict__ scales) {
-  __shared__ uint32_t part[kQuantThreads / 32];
-  for (long r = blockIdx.x; r < R; r += gridDim.x) {
+__device__ __forceinline__ float scale_of(uint32_t bits) {      // of a row whose largest magnitude has these bits
+  return bits < 0x7f800000u ? __uint_as_float(bits) / 127.0f : __uint_as_float(0x7fc00000u);
+}
+
+// The largest of the team's values; every thread gets it. `part`, `turn`: as team_sums has them.
+template <int TEAM>
+__device__ __forceinline__ uint32_t team_max(uint32_t m, uint32_t* part, int turn) {
+  if constexpr (TEAM >= 32) m = __reduce_max_sync(0xffffffffu, m);
+  else
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if constexpr (TEAM > 32) {
+    constexpr int kWarps = TEAM / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t* at = part + turn * (team_block<TEAM>() / 32);
+    if (lane == 0) at[warp] = m;
+    __syncthreads();
+    m = __reduce_max_sync(0xffffffffu, at[warp / kWarps * kWarps + (lane & (kWarps - 1))]);
+  }
+  return m;
+}
+
+// A team holds a row, like layer norm's; the next row's loads are under way meanwhile. Bound by the bytes of x.
+template <int VEC, int N, int TEAM>
+__global__ void __launch_bounds__(team_block<TEAM>()) quantize_rows_kernel(const float* __restrict__ x, long R, int C, int Cp, int8_t* __restrict__ codes,
+                                                                           float* __restrict__ scales) {
+  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  typedef Pack<int8_t, VEC> P;
+  __shared__ uint32_t part[2 * (kBlock / 32)];
+  const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+  const long step = (long)gridDim.x * kTeams;
+  long r = (long)blockIdx.x * kTeams + team;
+  Row<float, VEC, N, TEAM> row, next;
+  if (r < R) next.load(x + r * C, C, t, 0.f);
+  int turn = 0;
+  for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step, turn ^= 1) {
+    row = next;
+    if (r + step < R) next.load(x + (r + step) * C, C, t, 0.f);
     uint32_t m = 0;   // as whole numbers the bits of |x| order like the values, infinities and NaN above all
-    for (long c = threadIdx.x; c < C; c += kQuantThreads) m = max(m, __float_as_uint(x[r * C + c]) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, part[w]);
-    const bool finite = m < 0x7f800000u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(row.v[e]) & 0x7fffffffu);
+    m = team_max<TEAM>(m, part, turn);
+    if (r < R) {
+      const bool some = m != 0 && m < 0x7f800000u;
+      const float largest = __uint_as_float(m), inverse = 127.0f / largest;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * TEAM + t) * VEC;
+        if (c < Cp) {
+          P p;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) p.v[j] = (int8_t)(some ? (int)code_of(row.v[i * VEC + j], largest, inverse) : 0);
+          *reinterpret_cast<P*>(codes + r * Cp + c) = p;
+        }
+      }
+      if (t == 0) scales[r] = scale_of(m);
+    }
+  }
+}
+
+// rows that no team holds: read twice
+__global__ void __launch_bounds__(kLongThreads) quantize_rows_long_kernel(const float* __restrict__ x, long R, long C, long Cp, int8_t* __restrict__ codes,
+                                                                          float* __restrict__ scales) {
+  __shared__ uint32_t part[2 * 32];
+  int turn = 0;
+  for (long r = blockIdx.x; r < R; r += gridDim.x, turn ^= 1) {
+    uint32_t m = 0;
+    for (long c = threadIdx.x; c < C; c += kLongThreads) m = max(m, __float_as_uint(x[r * C + c]) & 0x7fffffffu);
+    m = team_max<kLongThreads>(m, part, turn);
+    const bool some = m != 0 && m < 0x7f800000u;
     const float largest = __uint_as_float(m), inverse = 127.0f / largest;
-    for (long c = threadIdx.x; c < Cp; c += kQuantThreads)
-      codes[r * Cp + c] = (int8_t)(c < C && finite && m != 0 ? code_of(x[r * C + c], largest, inverse) : 0.0f);
-    if (threadIdx.x == 0) scales[r] = finite ? largest / 127.0f : __uint_as_float(0x7fc00000u);
+    for (long c = threadIdx.x; c < Cp; c += kLongThreads)
+      codes[r * Cp + c] = (int8_t)(c < C && some ? (int)code_of(x[r * C + c], largest, inverse) : 0);
+    if (threadIdx.x == 0) scales[r] = scale_of(m);
   }
 }
 
@@ -579,12 +676,8 @@ CGTB_API int cgtb_dropout(int dtype, const void* x, long n, double p, const int6
   const double t = std::nearbyint(p * 4294967296.0);
   const uint32_t threshold = t >= 4294967295.0 ? 4294967295u : (uint32_t)t;
   const double scale = 1.0 / (1.0 - p);
-  const long blocks = cgtb_ceil_div(cgtb_ceil_div(n, 4), 256);
-  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
-  if (dtype == cgtb_f4)
-    CGTB_LAUNCH(dropout_kernel<float>, grid, 256, 0, (const float*)x, n, threshold, (float)scale, (const long*)state, site, (float*)y);
-  else
-    CGTB_LAUNCH(dropout_kernel<double>, grid, 256, 0, (const double*)x, n, threshold, scale, (const long*)state, site, (double*)y);
+  if (dtype == cgtb_f4) dropout((const float*)x, n, threshold, scale, state, site, (float*)y);
+  else dropout((const double*)x, n, threshold, scale, state, site, (double*)y);
   CGTB_CHECK_LAUNCH("dropout");
   return 0;
 }
@@ -593,8 +686,19 @@ CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, f
   if (!require_runtime("cgtb_quantize_rows")) return 1;
   if (R < 0 || C < 0) return fail("cgtb_quantize_rows: negative extent");
   if (R == 0) return 0;
-  const unsigned grid = (unsigned)(R < 65536 ? R : 65536);
-  CGTB_LAUNCH(quantize_rows_kernel, grid, kQuantThreads, 0, x, R, C, cgtb_ceil_div(C, 16) * 16, codes, scales);
+  const long Cp = cgtb_ceil_div(C, 16) * 16;
+  const bool wide = starts_on_16<float>(C, {x});
+  const bool held = with_team<16, 1024>(Cp, [&](auto team) {
+    constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
+    auto launch = [&](auto width) {
+      constexpr auto kernel = quantize_rows_kernel<decltype(width)::value, 16 / decltype(width)::value, TEAM>;
+      const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
+      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, R, (int)C, (int)Cp, codes, scales);
+    };
+    if (wide) launch(std::integral_constant<int, 4>());
+    else launch(std::integral_constant<int, 1>());
+  });
+  if (!held) CGTB_LAUNCH(quantize_rows_long_kernel, (unsigned)std::min<long>(R, rt().sm_count * 2L), kLongThreads, 0, x, R, C, Cp, codes, scales);
   CGTB_CHECK_LAUNCH("quantize_rows");
   return 0;
 }
