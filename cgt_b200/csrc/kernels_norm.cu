@@ -498,7 +498,7 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
 // A thread makes UNROLL blocks of four words, their elements loaded beforehand, 16 bytes at a time where the arrays start on
 // 16-byte boundaries. Bound by the bytes of x and y; the ten rounds of a block are forty multiplications for four elements.
 template <typename T, bool WIDE, int UNROLL>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* x, long n, uint32_t threshold, T scale, const long* __restrict__ state,
+__global__ void __launch_bounds__(256, 6) dropout_kernel(const T* x, long n, uint32_t threshold, T scale, const long* __restrict__ state,
                                                       uint32_t site, T* y) {
   constexpr int kPack = WIDE ? 16 / sizeof(T) : 1, kPacks = 4 / kPack;
   typedef Pack<T, kPack> P;
@@ -542,11 +542,12 @@ template <typename T>
 void dropout(const T* x, long n, uint32_t threshold, double scale, const int64_t* state, unsigned site, T* y) {
   const bool wide = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
   const long blocks = cgtb_ceil_div(cgtb_ceil_div(n, 4), 256);
-  auto launch = [&](auto kernel) {
-    CGTB_LAUNCH(kernel, (unsigned)std::min<long>(blocks, rt().sm_count * 8L), 256, 0, x, n, threshold, (T)scale, (const long*)state, site, y);
+  auto launch = [&](auto wide16) {
+    constexpr auto kernel = dropout_kernel<T, decltype(wide16)::value, 2>;
+    CGTB_LAUNCH(kernel, (unsigned)std::min(blocks, resident_blocks<kernel, 256, 0>()), 256, 0, x, n, threshold, (T)scale, (const long*)state, site, y);
   };
-  if (wide) launch(dropout_kernel<T, true, 2>);
-  else launch(dropout_kernel<T, false, 2>);
+  if (wide) launch(std::true_type());
+  else launch(std::false_type());
 }
 
 // ================================================================================================
@@ -554,13 +555,27 @@ void dropout(const T* x, long n, uint32_t threshold, double scale, const int64_t
 // ================================================================================================
 
 // The exact code of x: the quotient of two numbers of 31 and 24 bits is never rounded across a tie in 64 bits.
-__device__ __noinline__ float code_exact(float x, float largest) { return (float)rint(127.0 * (double)x / (double)largest); }
+__device__ __noinline__ int code_exact(float x, float largest) { return (int)rint(127.0 * (double)x / (double)largest); }
 
-// `inverse` = 127 / largest in 32 bits. x * inverse is off by less than 127 * 2^-22 = 3e-5: wherever it is not that near to a
-// tie, its nearest whole number is the exact quotient's.
-__device__ __forceinline__ float code_of(float x, float largest, float inverse) {
-  const float t = x * inverse, k = rintf(t);
-  return fabsf(t - k) < 0.4999f ? k : code_exact(x, largest);   // also for an inverse that overflows: then t is not finite
+// The codes of VEC elements in the low bytes of a word. `inverse` = 127 / largest in 32 bits: x * inverse is off by less than
+// 127 * 2^-22 = 3e-5, so wherever it is not that near to a tie, its nearest whole number is the exact quotient's. Adding
+// 1.5 * 2^23 rounds to that number, ties to even, and leaves it in the low bits: no conversion, whose pipe would bound the kernel.
+template <int VEC>
+__device__ __forceinline__ uint32_t codes_of(const float* x, float largest, float inverse, bool exact) {
+  constexpr float kRound = 12582912.0f;
+  uint32_t w[VEC];
+  float off = 0.f;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const float t = __fmul_rn(x[j], inverse), k = __fadd_rn(t, kRound);
+    off = fmaxf(off, fabsf(__fadd_rn(t, -__fadd_rn(k, -kRound))));
+    w[j] = __float_as_uint(k);
+  }
+  if (off >= 0.4999f || exact)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[j] = (uint32_t)code_exact(x[j], largest);
+  if constexpr (VEC == 1) return w[0];
+  else return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ float scale_of(uint32_t bits) {      // of a row whose largest magnitude has these bits
@@ -590,7 +605,6 @@ template <int VEC, int N, int TEAM>
 __global__ void __launch_bounds__(team_block<TEAM>()) quantize_rows_kernel(const float* __restrict__ x, long R, int C, int Cp, int8_t* __restrict__ codes,
                                                                            float* __restrict__ scales) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
-  typedef Pack<int8_t, VEC> P;
   __shared__ uint32_t part[2 * (kBlock / 32)];
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   const long step = (long)gridDim.x * kTeams;
@@ -608,14 +622,25 @@ __global__ void __launch_bounds__(team_block<TEAM>()) quantize_rows_kernel(const
     if (r < R) {
       const bool some = m != 0 && m < 0x7f800000u;
       const float largest = __uint_as_float(m), inverse = 127.0f / largest;
+      const bool exact = !(inverse <= 3.0e38f);      // rows of the smallest numbers
+      uint32_t w[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = (i * TEAM + t) * VEC;
-        if (c < Cp) {
-          P p;
+      for (int i = 0; i < N; ++i) w[i] = some ? codes_of<VEC>(row.v + i * VEC, largest, inverse, exact) : 0u;
+      if constexpr (TEAM == 1 && VEC == 1 && N == 16) {     // the whole row is this thread's
+        uint4 all;
+        uint32_t* q = &all.x;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) p.v[j] = (int8_t)(some ? (int)code_of(row.v[i * VEC + j], largest, inverse) : 0);
-          *reinterpret_cast<P*>(codes + r * Cp + c) = p;
+        for (int i = 0; i < 4; ++i)
+          q[i] = __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0040), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0040), 0x5410);
+        *reinterpret_cast<uint4*>(codes + r * Cp) = all;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = (i * TEAM + t) * VEC;
+          if (c < Cp) {
+            if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(codes + r * Cp + c) = w[i];
+            else codes[r * Cp + c] = (int8_t)w[i];
+          }
         }
       }
       if (t == 0) scales[r] = scale_of(m);
@@ -635,7 +660,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_rows_long_kernel(const 
     const bool some = m != 0 && m < 0x7f800000u;
     const float largest = __uint_as_float(m), inverse = 127.0f / largest;
     for (long c = threadIdx.x; c < Cp; c += kLongThreads)
-      codes[r * Cp + c] = (int8_t)(c < C && some ? (int)code_of(x[r * C + c], largest, inverse) : 0);
+      codes[r * Cp + c] = (int8_t)(c < C && some ? codes_of<1>(x + r * C + c, largest, inverse, !(inverse <= 3.0e38f)) : 0u);
     if (threadIdx.x == 0) scales[r] = scale_of(m);
   }
 }
