@@ -147,6 +147,20 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
   }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a value of another block of the cluster, whose shared memory is laid out like this one's
+template <typename T>
+__device__ __forceinline__ T load_remote(uint32_t local, int rank) {
+  T v;
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  if constexpr (sizeof(T) == 4) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  else asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // One element group of a thread from global to shared memory, asynchronously
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from) {
@@ -166,10 +180,10 @@ constexpr int kAhead = 2;
 template <typename T, int VEC, int N, int TEAM>
 constexpr size_t norm_backward_bytes() { return (size_t)(kAhead + 1) * 2 * N * team_block<TEAM>() * VEC * sizeof(T); }
 
-template <typename T, int VEC, int N, int TEAM>
+template <typename T, int VEC, int N, int TEAM, bool ONE>
 __global__ void __launch_bounds__(team_block<TEAM>(), (TEAM == 1024 || VEC * N * sizeof(T) == 32 && sizeof(T) == 4 ? 1024 : 512) / team_block<TEAM>())
 norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy, long R, int C, T eps, T* __restrict__ dx,
-                     T* __restrict__ part) {
+                     T* __restrict__ part, T* __restrict__ dgain, T* __restrict__ dbias) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
   typedef Pack<T, VEC> P;
   extern __shared__ __align__(16) unsigned char ahead_raw[];
@@ -249,15 +263,17 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       a.store(dx + r * C, C, t);
     }
   }
-  T* out = part + (long)blockIdx.x * 2 * C;
-  T* joined = reinterpret_cast<T*>(ahead_raw);      // 2 E of the block's threads: less than the rows took
+  // ONE, for few rows: the whole grid is one cluster, whose blocks leave their sums in their shared memory and then add all
+  // blocks' sums of a share of the columns, in order; no second kernel.
+  T* joined = reinterpret_cast<T*>(ahead_raw);      // 2 E of the block's threads, or 2 C: less than the rows took
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (kTeams > 1 || ONE) __syncthreads();
+  T* out = ONE ? joined + (kTeams > 1 ? 2 * E * kBlock : 0) : part + (long)blockIdx.x * 2 * C;
   if (kTeams == 1) {
     dg.store(out, C, t);
     db.store(out + C, C, t);
   } else {
     // [e][thread]; then the columns are added over the teams, in order
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       joined[(2 * e) * kBlock + threadIdx.x] = dg.v[e];
@@ -272,29 +288,55 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       if (c < C) out[(long)which * C + c] = v;
     }
   }
+  if constexpr (ONE) {
+    cluster_sync();
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(out);
+    for (int c = blockIdx.x * kBlock + threadIdx.x; c < 2 * C; c += gridDim.x * kBlock) {
+      T v = T(0);
+      for (int q = 0; q < (int)gridDim.x; ++q) v += load_remote<T>(at + c * (uint32_t)sizeof(T), q);
+      if (c < C) dgain[c] = v;
+      else dbias[c - C] = v;
+    }
+    cluster_sync();      // the others have read this block's sums
+  }
 }
 
-// dgain and dbias from the blocks' sums part[P][2][C]: 32 of the 2 C columns per block, 32 groups of threads that each add
-// every 32nd block's, then the groups in order
+// dgain and dbias from the blocks' sums part[P][2][C]: 32 groups of VEC of the 2 C columns per block, 32 warps that each add
+// every 32nd block's, then the warps' sums in order
 constexpr int kFoldGroups = 32;
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kFoldGroups) norm_fold_kernel(const T* __restrict__ part, long C, int P, T* __restrict__ dgain, T* __restrict__ dbias) {
-  __shared__ T joined[kFoldGroups][32];
+  typedef Pack<T, VEC> V;
+  __shared__ V joined[kFoldGroups][32];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
-  const long c = (long)blockIdx.x * 32 + lane;
-  T s = T(0);
+  const long c = ((long)blockIdx.x * 32 + lane) * VEC;
+  V s;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) s.v[j] = T(0);
   if (c < 2 * C) {
-#pragma unroll 8
-    for (int q = group; q < P; q += kFoldGroups) s += part[(long)q * 2 * C + c];
+#pragma unroll 4
+    for (int q = group; q < P; q += kFoldGroups) {
+      const V v = *reinterpret_cast<const V*>(part + (long)q * 2 * C + c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s.v[j] += v.v[j];
+    }
   }
   joined[group][lane] = s;
   __syncthreads();
-  if (group == 0 && c < 2 * C) {
+  if (group < VEC && c - lane * VEC < 2 * C) {       // warp j adds column j of every group of columns
+    const long mine = c + group;
+    T v = joined[0][lane].v[group];
 #pragma unroll
-    for (int q = 1; q < kFoldGroups; ++q) s += joined[q][lane];
-    if (c < C) dgain[c] = s;
-    else dbias[c - C] = s;
+    for (int q = 1; q < kFoldGroups; ++q) v += joined[q][lane].v[group];
+    if (mine < C) dgain[mine] = v;
+    else if (mine < 2 * C) dbias[mine - C] = v;
   }
+}
+template <typename T>
+void norm_fold(const T* part, long C, long P, T* dgain, T* dbias) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (2 * C % VEC == 0) CGTB_LAUNCH((norm_fold_kernel<T, VEC>), (unsigned)cgtb_ceil_div(2 * C, 32 * VEC), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
+  else CGTB_LAUNCH((norm_fold_kernel<T, 1>), (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
 }
 
 // ---- longer rows, up to 20480 float32 or 10240 float64: a block of 1024 threads holds one, 20 or 10 elements a thread, and has
@@ -547,27 +589,48 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   return 0;
 }
 
-// The gradients by teams of E elements a thread: the rows' sums in `part` for P blocks. 1: failed, -1: no team is that large
+// The gradients by teams of E elements a thread; dgain and dbias are complete, or in `part` for P blocks. 1: failed, -1: no team
+// is that large
 template <typename T, int E, int kMaxTeam>
-int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T*& part, long& P) {
+int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias, T*& part, long& P) {
   const bool wide = starts_on_16<T>(C, {x, gain, gy, dx});
+  int failed = 0;
   const bool held = with_team<E, kMaxTeam>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
     auto launch = [&](auto width) {
       constexpr int VEC = decltype(width)::value;
       constexpr size_t bytes = norm_backward_bytes<T, VEC, E / VEC, TEAM>();
-      constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM>;
+      constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM, false>, one = norm_backward_kernel<T, VEC, E / VEC, TEAM, true>;
+      const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
+      if (steps <= 32) {      // a cluster of eight blocks makes up to four steps each: less than another kernel takes
+        (void)resident_blocks<one, kBlock, bytes>();      // allows the shared memory
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = steps > 4 ? 8 : steps > 2 ? 4 : steps > 1 ? 2 : 1;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(attr.val.clusterDim.x);
+        config.blockDim = dim3(kBlock);
+        config.dynamicSmemBytes = bytes;
+        config.stream = rt().stream;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias);
+        if (e != cudaSuccess) failed = fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e));
+        g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+        return;
+      }
       // at least four rows for a team, so that what the blocks leave for the last kernel stays small against the rows; but no SM
       // without a block where there are rows for it
-      const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
       P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
       part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
-      if (part) CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part);
+      if (!part) failed = 1;
+      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr);
     };
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
     else launch(std::integral_constant<int, 1>());
   });
-  return !held ? -1 : part ? 0 : 1;
+  return held ? failed : -1;
 }
 
 template <typename T>
@@ -578,8 +641,8 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   // warps too few rows are under way at a time (8192 x 4096: 79 us with 8, 85 us with 16), with float64 registers run out
   // (8192 x 1024: 46 us with 4, 51 us with 8)
   int failed;
-  if (sizeof(T) == 4 && C > 16 && C <= 2048) failed = norm_backward_teams<T, 16, 128>(x, gain, gy, R, C, eps, dx, part, P);
-  else failed = norm_backward_teams<T, 32 / sizeof(T), 1024>(x, gain, gy, R, C, eps, dx, part, P);
+  if (sizeof(T) == 4 && C > 16 && C <= 2048) failed = norm_backward_teams<T, 16, 128>(x, gain, gy, R, C, eps, dx, dgain, dbias, part, P);
+  else failed = norm_backward_teams<T, 32 / sizeof(T), 1024>(x, gain, gy, R, C, eps, dx, dgain, dbias, part, P);
   if (failed > 0) return 1;
   if (failed < 0 && C <= kLongThreads * wide_elements<T>()) {
     auto launch = [&](auto width) {
@@ -603,7 +666,7 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     CGTB_LAUNCH(norm_backward_long_kernel<T>, (unsigned)grid, kLongThreads, 0, x, gain, gy, R, C, (T)eps, dx, stats);
     CGTB_LAUNCH(norm_columns_kernel<T>, dim3((unsigned)cblocks, (unsigned)P), 256, 0, x, gy, stats, R, C, cgtb_ceil_div(R, P), part);
   }
-  CGTB_LAUNCH(norm_fold_kernel<T>, (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
+  if (part) norm_fold(part, C, P, dgain, dbias);
   CGTB_CHECK_LAUNCH("layer_norm_backward");
   return 0;
 }
