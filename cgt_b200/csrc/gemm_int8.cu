@@ -26,7 +26,7 @@ struct Params {
   float* y;
   long M, N, K;
   int BN, stages, tmem_cols, a_bytes;
-  int mtiles, ntiles;
+  int mtiles, ntiles, tile_rows;
   long total;
   int vec;
   int split, split_log;             // CTAs of a cluster that share a tile, a power of two
@@ -38,12 +38,12 @@ struct Tile { long m0, n0; };
 __device__ __forceinline__ Tile tile_of(const Params& p, long t) {
   const long per = (long)kGroup * p.ntiles, g = t / per, first = g * kGroup;
   const long rows = p.mtiles - first < kGroup ? p.mtiles - first : kGroup, r = t - g * per;
-  return Tile{(first + r % rows) * kRows, (r / rows) * p.BN};
+  return Tile{(first + r % rows) * p.tile_rows, (r / rows) * p.BN};
 }
 
 // D 32-bit integers, A and B signed 8-bit integers, both K-major
-__device__ __forceinline__ uint32_t idesc_int8(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+__device__ __forceinline__ uint32_t idesc_int8(int n, int m = kRows) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_int8(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -73,6 +73,14 @@ __device__ __forceinline__ bool wait_sleeping(uint32_t bar, uint32_t parity, con
   ok = __shfl_sync(0xffffffffu, ok, 0);
   if (ok) (void)mbar_try(bar, parity);   // every lane observes the phase itself
   return ok != 0;
+}
+
+// The epilogue warps go on together or not at all: they meet at a barrier in every tile, where none may be missing.
+__device__ __forceinline__ bool epilogue_agrees(bool ok) {
+  uint32_t failed;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.eq.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(failed) : "r"((uint32_t)ok), "n"(kEpilogueWarps * 32) : "memory");
+  return failed == 0;
 }
 
 // Word offset of quad q of row `row` in a warp's 32 x 16 block: 16-byte accesses by rows and by quads without bank conflicts
@@ -213,9 +221,8 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         if (lane == 0) { *(volatile int*)p.err = 3; __threadfence_system(); }
       }
       if (SPLIT) break;
-      // the epilogue warps go on together: they meet at a barrier in every tile
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
-      if (*abortp) { ok = false; break; }
+      ok = epilogue_agrees(ok);
+      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (int ch = half; m0 < p.M && ch < p.BN / 16; ch += 2) {
         uint32_t r[16];
@@ -336,6 +343,181 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Large products: two CTAs of a cluster, on two SMs, share tiles of 256 x 256 results (tcgen05 cta_group::2). Each loads its 128
+// rows of a and 128 of the 256 rows of b, and holds its 128 rows of sums in its TMEM; the even CTA's MMA thread issues for both,
+// and every tensor core reads both halves of b. A stage is 32 KB in either SM instead of 48 KB: the L2 cache, whose bandwidth
+// bounds the kernel above (a stage took 630 cycles, its MMAs 512), delivers a third less, and six stages fit instead of four.
+// 8192 x 4096 x 4096: PAUSE us.
+//
+// Barriers: `full` is the even CTA's, told by the loads of both; `empty` and `acc_full` are each CTA's own, told by the MMAs'
+// commits, which go to both; `acc_empty` is the even CTA's, told by the epilogue warps of both.
+// ------------------------------------------------------------------------------------------------
+constexpr int kPairRows = 256;
+
+__device__ __forceinline__ void mma_int8_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives at the barriers at this place in both CTAs when the MMAs issued so far have run
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// into this CTA's memory; the bytes are counted at the barrier of the pair's even CTA (`bar`: an address of the cluster window)
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ bool try_cluster(uint32_t bar, uint32_t parity) {   // sees what the other CTA released
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+int8_product_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(16) float columns[2 * 512];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t kHalf = 128 * kDepth, kStage = 2 * kHalf;
+  volatile int* abortp = &abort_flag;
+  const uint32_t rank = cluster_rank();
+  const long t_first = blockIdx.x >> 1, t_step = gridDim.x >> 1;
+  const int nkb = (int)((p.K + kDepth - 1) / kDepth);
+
+  if (tid < p.stages) {
+    mbar_init(smem_u32(&full[tid]), 2);            // the even CTA's two loading threads, which announce the other's bytes too
+    mbar_init(smem_u32(&empty[tid]), 1);
+  }
+  if (tid == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&acc_full[b]), 1);
+      mbar_init(smem_u32(&acc_empty[b]), 2 * kEpilogueWarps);
+    }
+    abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
+  }
+  if (warp == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (warp == kEpilogueWarps) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp < kEpilogueWarps) {
+    const int quarter = warp & 3, half = warp >> 2;
+    float* block = reinterpret_cast<float*>(smem + p.block_offset) + warp * 512;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint32_t it = 0;
+    for (long t = t_first; t < p.total; t += t_step, ++it) {
+      const Tile c = tile_of(p, t);
+      const uint32_t buf = it & 1u;
+      const long m0 = c.m0 + (long)rank * 128 + quarter * 32;
+      const float row_scale = m0 + lane < p.M ? p.sa[m0 + lane] : 0.f;
+      const float* scales = stage_columns(p, columns, it, c.n0, tid);
+      ok = wait_sleeping(smem_u32(&acc_full[buf]), (it >> 1) & 1u, abortp, lane);
+      if (!ok) {
+        *abortp = 1;
+        if (lane == 0) { *(volatile int*)p.err = 3; __threadfence_system(); }
+      }
+      ok = epilogue_agrees(ok);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int ch = half; m0 < p.M && ch < 16; ch += 2) {
+        uint32_t r[16];
+        tmem_ld16(lanes + buf * 256u + (uint32_t)ch * 16u, r);
+        store_chunk(p, r, row_scale, m0, c.n0 + ch * 16, block, scales + ch * 16, lane);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_address(smem_u32(&acc_empty[buf]), 0u)) : "memory");
+    }
+  } else if (warp == kEpilogueWarps) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = idesc_int8(256, kPairRows), base = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+      const uint64_t da0 = make_desc(base), db0 = make_desc(base + kHalf);
+      uint32_t s = 0, phase = 0, it = 0;
+      for (long t = t_first; t < p.total && ok; t += t_step, ++it) {
+        const uint32_t buf = it & 1u, bar = smem_u32(&acc_empty[buf]), parity = ((it >> 1) & 1u) ^ 1u;
+        ok = mbar_wait_or_abort(bar, parity, abortp) && try_cluster(bar, parity);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + buf * 256u;
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_or_abort(full0 + 8u * s, phase, abortp);
+          if (!ok) break;
+          const uint64_t da = da0 + s * (kStage >> 4), db = db0 + s * (kStage >> 4);
+          mma_int8_pair(d, da, db, idesc, kb > 0);
+          mma_int8_pair(d, da + 2, db + 2, idesc, 1u);
+          mma_int8_pair(d, da + 4, db + 4, idesc, 1u);
+          mma_int8_pair(d, da + 6, db + 6, idesc, 1u);
+          mma_commit_pair(empty0 + 8u * s);
+          if (++s == (uint32_t)p.stages) { s = 0; phase ^= 1u; }
+        }
+        if (ok) mma_commit_pair(smem_u32(&acc_full[buf]));
+      }
+      if (!ok) { *abortp = 1; *(volatile int*)p.err = 4; __threadfence_system(); }
+    }
+    __syncwarp();
+  } else {
+    if (elect_one()) {
+      const bool is_b = warp == kEpilogueWarps + 2;
+      const CUtensorMap* map = is_b ? &map_b : &map_a;
+      const uint32_t dst0 = smem_u32(smem) + (is_b ? kHalf : 0u), empty0 = smem_u32(empty), full0 = remote_address(smem_u32(full), 0u);
+      uint32_t issued = 0, s = 0, phase = 1;
+      for (long t = t_first; t < p.total && ok; t += t_step) {
+        const Tile c = tile_of(p, t);
+        const int row = (int)((is_b ? c.n0 : c.m0) + (long)rank * 128);
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_or_abort(empty0 + 8u * s, phase, abortp);
+          if (!ok) break;
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(full) + 8u * s, 2 * kHalf);
+          load_2d_pair(dst0 + s * kStage, map, kb * kDepth, row, full0 + 8u * s);
+          ++issued;
+          if (++s == (uint32_t)p.stages) { s = 0; phase ^= 1u; }
+        }
+      }
+      // Copies still write this CTA's memory until the MMAs have read them; before the CTA leaves, every stage issued has to be
+      // empty again (bounded; when a wait has expired somewhere, this one does too).
+      const uint32_t stages = (uint32_t)p.stages;
+      for (uint32_t j = (issued > stages ? issued - stages : 0u); j != issued && ok; ++j) ok = mbar_wait_or_abort(empty0 + 8u * (j % stages), (j / stages) & 1u, abortp);
+      if (!ok || *abortp) {
+        *abortp = 1;
+        *(volatile int*)p.err = 5;
+        __threadfence_system();
+        const long long t0 = clock64();      // whatever is in flight lands meanwhile
+        while (clock64() - t0 < 2000000) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();        // neither CTA leaves while the other reads its memory or tells its barriers
+  if (warp == kEpilogueWarps) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -381,38 +563,44 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
       if (best < 0 || cost < best) { best = cost; p.BN = bn; p.split = split; p.split_log = log; }
     }
   }
+  // Pairs of CTAs, where their larger tiles leave none without work
+  const bool pairs = p.split == 1 && p.BN == 256 && M > kRows && cgtb_ceil_div(M, kPairRows) * cgtb_ceil_div(N, 256) >= sms / 2;
+  p.tile_rows = pairs ? kPairRows : kRows;
+  p.mtiles = (int)cgtb_ceil_div(M, p.tile_rows);
   p.ntiles = (int)cgtb_ceil_div(N, p.BN);
   p.total = (long)p.mtiles * p.ntiles;
   p.tmem_cols = (p.split > 1 ? 1 : 2) * p.BN;
   const int a_rows = (int)std::min<long>(kRows, cgtb_ceil_div(M, 8) * 8);
   p.a_bytes = a_rows * kDepth;
   p.vec = N % 4 == 0 && ((uintptr_t)y & 15) == 0;
-  const int stage_bytes = p.a_bytes + p.BN * kDepth, epilogue = kEpilogueWarps * 512 * 4;
+  const int box_b = pairs ? 128 : p.BN, stage_bytes = p.a_bytes + box_b * kDepth, epilogue = kEpilogueWarps * 512 * 4;
   p.stages = std::min(kMaxStages, (220 * 1024 - 1024 - epilogue) / stage_bytes);
   if (p.split > 1) p.stages = std::min(p.stages, (int)cgtb_ceil_div(nkb, p.split));
   const int slots = (p.split - 1) * (int)cgtb_ceil_div(p.BN / 32, p.split) * kSlotBytes;
   p.block_offset = std::max(p.stages * stage_bytes, slots);
   const int smem = 1024 + p.block_offset + epilogue;
   CUtensorMap map_a, map_b;
-  if (!encode(&map_a, a, M, K, a_rows) || !encode(&map_b, b, N, K, p.BN)) return fail("cgtb_int8_product: no tensor map for %ld x %ld x %ld", M, N, K);
+  if (!encode(&map_a, a, M, K, a_rows) || !encode(&map_b, b, N, K, box_b)) return fail("cgtb_int8_product: no tensor map for %ld x %ld x %ld", M, N, K);
   static const cudaError_t attribute = [] {
     const cudaError_t e = cudaFuncSetAttribute(int8_product_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(int8_product_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    if (e != cudaSuccess) return e;
+    const cudaError_t f = cudaFuncSetAttribute(int8_product_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(int8_product_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
   }();
   if (attribute != cudaSuccess) return fail("cgtb_int8_product: %s", cudaGetErrorString(attribute));
-  if (p.split > 1) {
+  if (p.split > 1 || pairs) {
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)p.split;
+    attr.val.clusterDim.x = pairs ? 2u : (unsigned)p.split;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(p.total * p.split));
+    config.gridDim = dim3((unsigned)(pairs ? 2 * std::min<long>(p.total, sms / 2) : p.total * p.split));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = (size_t)smem;
     config.stream = rt().stream;
     config.attrs = &attr;
     config.numAttrs = 1;
-    CGTB_CUDA_TRY(cudaLaunchKernelEx(&config, int8_product_tc_kernel<true>, map_a, map_b, p));
+    CGTB_CUDA_TRY(cudaLaunchKernelEx(&config, pairs ? int8_product_pair_kernel : int8_product_tc_kernel<true>, map_a, map_b, p));
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   } else {
     CGTB_LAUNCH(int8_product_tc_kernel<false>, (unsigned)std::min<long>(p.total, sms), kThreads, smem, map_a, map_b, p);
