@@ -75,6 +75,22 @@ __device__ __forceinline__ bool wait_sleeping(uint32_t bar, uint32_t parity, con
   return ok != 0;
 }
 
+// 16 columns of this warp's 32 lanes of TMEM; the registers hold them after tmem_arrived()
+__device__ __forceinline__ void tmem_request16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+
 // The epilogue warps go on together or not at all: they meet at a barrier in every tile, where none may be missing.
 __device__ __forceinline__ bool epilogue_agrees(bool ok) {
   uint32_t failed;
@@ -129,14 +145,37 @@ __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)
     }
   }
 }
-// the scales and biases of a tile's columns, brought to shared memory while the tile's sums are formed; `it`: two places
-__device__ __forceinline__ const float* stage_columns(const Params& p, float* columns, uint32_t it, long n0, int tid) {
-  float* to = columns + (it & 1u) * 512;
-  const long n = n0 + tid;
-  if (tid < p.BN) {
-    to[tid] = n < p.N ? p.sb[n] : 0.f;
-    to[256 + tid] = n < p.N && p.bias ? p.bias[n] : 0.f;
+// A warp's share of a tile: its 32 rows, every other chunk of 16 columns. The next chunk is on its way from TMEM meanwhile;
+// release() is called when nothing more is read there.
+template <typename F>
+__device__ __forceinline__ void store_tile_rows(const Params& p, uint32_t taddr, int chunks, int half, float row_scale, long m0, long n0, float* block,
+                                                const float* scales, int lane, F release) {
+  uint32_t r[16], next[16];
+  if (half < chunks) tmem_request16(taddr + (uint32_t)half * 16u, next);
+  for (int ch = half; ch < chunks; ch += 2) {
+    tmem_arrived(next);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = next[j];
+    if (ch + 2 < chunks) tmem_request16(taddr + (uint32_t)(ch + 2) * 16u, next);
+    else {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      release();
+    }
+    store_chunk(p, r, row_scale, m0, n0 + ch * 16, block, scales + ch * 16, lane);
   }
+}
+// What an epilogue thread brings to a tile: its row's scale, and the scale and bias of one column, which go to shared memory. They
+// are asked for a tile ahead.
+struct Scales { float row, column, bias; };
+__device__ __forceinline__ Scales ask_scales(const Params& p, long row, long n0, int tid) {
+  const long n = n0 + tid;
+  const bool inside = tid < p.BN && n < p.N;
+  return Scales{row < p.M ? p.sa[row] : 0.f, inside ? p.sb[n] : 0.f, inside && p.bias ? p.bias[n] : 0.f};
+}
+__device__ __forceinline__ const float* stage_columns(const Scales& s, float* columns, uint32_t it, int tid) {   // `it`: two places
+  float* to = columns + (it & 1u) * 512;
+  to[tid] = s.column;
+  to[256 + tid] = s.bias;
   asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
   return to;
 }
@@ -209,12 +248,17 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 
   if (warp < kEpilogueWarps) {
     uint32_t it = 0;
+    Tile c = tile_of(p, t_first);
+    Scales ahead = ask_scales(p, c.m0 + quarter * 32 + lane, c.n0, tid);
     for (long t = t_first; t < p.total; t += t_step, ++it) {
-      const Tile c = tile_of(p, t);
       const uint32_t buf = it & 1u;
-      const long m0 = c.m0 + quarter * 32;
-      row_scale = m0 + lane < p.M ? p.sa[m0 + lane] : 0.f;
-      const float* scales = stage_columns(p, columns, it, c.n0, tid);
+      const long m0 = c.m0 + quarter * 32, n0 = c.n0;
+      row_scale = ahead.row;
+      const float* scales = stage_columns(ahead, columns, it, tid);
+      if (!SPLIT && t + t_step < p.total) {
+        c = tile_of(p, t + t_step);
+        ahead = ask_scales(p, c.m0 + quarter * 32 + lane, c.n0, tid);
+      }
       ok = wait_sleeping(smem_u32(&acc_full[buf]), (it >> 1) & 1u, abortp, lane);
       if (!ok) {
         *abortp = 1;
@@ -224,14 +268,9 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       ok = epilogue_agrees(ok);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (int ch = half; m0 < p.M && ch < p.BN / 16; ch += 2) {
-        uint32_t r[16];
-        tmem_ld16(lanes + buf * (uint32_t)p.BN + (uint32_t)ch * 16u, r);
-        store_chunk(p, r, row_scale, m0, c.n0 + ch * 16, block, scales + ch * 16, lane);
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
+      auto release = [&] { if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf])); };
+      if (m0 < p.M) store_tile_rows(p, lanes + buf * (uint32_t)p.BN, p.BN / 16, half, row_scale, m0, n0, block, scales, lane, release);
+      else release();
     }
   } else if (warp == kEpilogueWarps) {
     // MMA issuer
@@ -425,12 +464,18 @@ int8_product_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     float* block = reinterpret_cast<float*>(smem + p.block_offset) + warp * 512;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     uint32_t it = 0;
+    const long own = (long)rank * 128 + quarter * 32;     // of a tile's rows
+    Tile c = tile_of(p, t_first);
+    Scales ahead = ask_scales(p, c.m0 + own + lane, c.n0, tid);
     for (long t = t_first; t < p.total; t += t_step, ++it) {
-      const Tile c = tile_of(p, t);
       const uint32_t buf = it & 1u;
-      const long m0 = c.m0 + (long)rank * 128 + quarter * 32;
-      const float row_scale = m0 + lane < p.M ? p.sa[m0 + lane] : 0.f;
-      const float* scales = stage_columns(p, columns, it, c.n0, tid);
+      const long m0 = c.m0 + own, n0 = c.n0;
+      const float row_scale = ahead.row;
+      const float* scales = stage_columns(ahead, columns, it, tid);
+      if (t + t_step < p.total) {
+        c = tile_of(p, t + t_step);
+        ahead = ask_scales(p, c.m0 + own + lane, c.n0, tid);
+      }
       ok = wait_sleeping(smem_u32(&acc_full[buf]), (it >> 1) & 1u, abortp, lane);
       if (!ok) {
         *abortp = 1;
@@ -439,15 +484,13 @@ int8_product_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       ok = epilogue_agrees(ok);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (int ch = half; m0 < p.M && ch < 16; ch += 2) {
-        uint32_t r[16];
-        tmem_ld16(lanes + buf * 256u + (uint32_t)ch * 16u, r);
-        store_chunk(p, r, row_scale, m0, c.n0 + ch * 16, block, scales + ch * 16, lane);
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_address(smem_u32(&acc_empty[buf]), 0u)) : "memory");
+      // relaxed: nothing in memory is handed over, and a release at cluster scope would wait for every store of results
+      auto release = [&] {
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_address(smem_u32(&acc_empty[buf]), 0u)) : "memory");
+      };
+      if (m0 < p.M) store_tile_rows(p, lanes + buf * 256u, 16, half, row_scale, m0, n0, block, scales, lane, release);
+      else release();
     }
   } else if (warp == kEpilogueWarps) {
     if (rank == 0 && elect_one()) {
