@@ -387,7 +387,8 @@ int8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 // rows of a and 128 of the 256 rows of b, and holds its 128 rows of sums in its TMEM; the even CTA's MMA thread issues for both,
 // and every tensor core reads both halves of b. A stage is 32 KB in either SM instead of 48 KB: the L2 cache, whose bandwidth
 // bounds the kernel above (a stage took 630 cycles, its MMAs 512), delivers a third less, and six stages fit instead of four.
-// 8192 x 4096 x 4096: PAUSE us.
+// 8192 x 4096 x 4096: 96 us in a row of calls (2.85 PFLOP/s; alone 89 us, the tensor pipe 85 % active at the 1.6 GHz that the
+// power cap leaves), 110 us by the kernel above.
 //
 // Barriers: `full` is the even CTA's, told by the loads of both; `empty` and `acc_full` are each CTA's own, told by the MMAs'
 // commits, which go to both; `acc_empty` is the even CTA's, told by the epilogue warps of both.
@@ -592,7 +593,7 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
   p.mtiles = (int)cgtb_ceil_div(M, kRows);
   // Widths and splits, by what they cost in cycles (measured): a stage takes 400 or, wide, two for each column; tiles follow each
   // other on an SM; a cluster's two barriers and its last step take 3000, what a CTA sends goes at 12 bytes a cycle. At
-  // 128 x 4096 x 4096 a width of 32 takes PAUSE us, 128 in clusters of four PAUSE us.
+  // 128 x 4096 x 4096 a width of 32 takes 14.5 us, 128 in clusters of four 11 us.
   const int nkb = (int)cgtb_ceil_div(K, kDepth), sms = rt().sm_count;
   long best = -1;
   for (int bn = 256; bn >= 32; bn /= 2) {
@@ -652,12 +653,97 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
   return 0;
 }
 
-// Few rows (one token at a time, up to eight): bound by the bytes of the weights. WARPS warps share an output channel, each lane
-// takes 16 codes of the channel's row at a time, four such loads in flight, and multiplies them with the codes of ROWS rows,
-// which come from the L1 cache; whole numbers are added by redux, in any order.
+// ------------------------------------------------------------------------------------------------
+// Small products and few rows, where the kernels above spend most of their time on beginning (5 to 8 us whatever they do). A
+// block makes 16 CT output channels x 8 NT rows; its eight warps take turns with 64 codes of K, UNROLL such steps in flight, and
+// join their sums in shared memory at the end. The weights are the matrix instructions' A operand (16 channels), the rows their
+// B operand (8 rows): with few rows nothing is multiplied in vain. No shared memory in the loop: which codes of K an instruction
+// sees in which of its places is free as long as both operands agree, so a thread loads 16 consecutive codes of a row and gives
+// them to two instructions as they are. Bound by latency, or by the bytes of the weights: 128 x 256 x 784 2.5 us,
+// 8 x 4096 x 4096 8.0 us (2.1 TB/s).
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int CT, int NT, int UNROLL>
+__global__ void __launch_bounds__(256) int8_product_small_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
+                                                                 const float* __restrict__ sb, const float* __restrict__ bias, long M, long N, long K,
+                                                                 float* __restrict__ y) {
+  constexpr int kChannels = 16 * CT, kTokens = 8 * NT, kPitch = kChannels + 1;
+  __shared__ int joined[8][kTokens * kPitch];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long n0 = (long)blockIdx.x * kChannels, m0 = (long)blockIdx.y * kTokens;
+  // rows beyond the operands are read as the last one: their results are not stored
+  const int8_t *w[2 * CT], *x[NT];
+#pragma unroll
+  for (int i = 0; i < 2 * CT; ++i) w[i] = b + (n0 + g + 8 * i < N ? n0 + g + 8 * i : N - 1) * K + t * 16;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) x[j] = a + (m0 + g + 8 * j < M ? m0 + g + 8 * j : M - 1) * K + t * 16;
+  int c[CT][NT][4];
+#pragma unroll
+  for (int i = 0; i < CT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[i][j][k] = 0;
+  const long last = K - t * 16;      // this thread's codes of a step are there for k < last
+  for (long k = warp * 64; k < K; k += 512 * UNROLL) {
+    uint4 wv[UNROLL][2 * CT], xv[UNROLL][NT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool there = k + u * 512 < last;
+#pragma unroll
+      for (int i = 0; i < 2 * CT; ++i) wv[u][i] = there ? __ldg(reinterpret_cast<const uint4*>(w[i] + k + u * 512)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) xv[u][j] = there ? __ldg(reinterpret_cast<const uint4*>(x[j] + k + u * 512)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_16832(c[i][j], wv[u][2 * i].x, wv[u][2 * i + 1].x, wv[u][2 * i].y, wv[u][2 * i + 1].y, xv[u][j].x, xv[u][j].y);
+          mma_16832(c[i][j], wv[u][2 * i].z, wv[u][2 * i + 1].z, wv[u][2 * i].w, wv[u][2 * i + 1].w, xv[u][j].z, xv[u][j].w);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < CT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) joined[warp][(8 * j + 2 * t + (k & 1)) * kPitch + 16 * i + 8 * (k >> 1) + g] = c[i][j][k];
+  __syncthreads();
+  const int channel = threadIdx.x % kChannels;
+  const long n = n0 + channel;
+  if (n < N) {
+    const float s = sb[n], shift = bias ? bias[n] : 0.f;
+    for (int token = threadIdx.x / kChannels; token < kTokens && m0 + token < M; token += 256 / kChannels) {
+      int sum = 0;
+#pragma unroll
+      for (int v = 0; v < 8; ++v) sum += joined[v][token * kPitch + channel];
+      const float r = (float)sum * sa[m0 + token] * s;
+      y[(m0 + token) * N + n] = bias ? r + shift : r;
+    }
+  }
+}
+
+template <int CT, int NT, int UNROLL>
+int product_small(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K, float* y) {
+  const dim3 grid((unsigned)cgtb_ceil_div(N, 16 * CT), (unsigned)cgtb_ceil_div(M, 8 * NT));
+  CGTB_LAUNCH((int8_product_small_kernel<CT, NT, UNROLL>), grid, 256, 0, a, sa, b, sb, bias, M, N, K, y);
+  CGTB_CHECK_LAUNCH("int8_product");
+  return 0;
+}
+
+// One row, a token at a time, or two: bound by the bytes of the weights. WARPS warps share an output channel, each lane takes 16
+// codes of the channel's row at a time, four such loads in flight, and multiplies them with the codes of ROWS rows, which come
+// from the L1 cache; whole numbers are added by redux, in any order. 1 x 8192 x 8192: 14.2 us, 4.7 TB/s.
 template <int ROWS, int WARPS>
-__global__ void __launch_bounds__(256) int8_product_rows_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
-                                                                const float* __restrict__ sb, const float* __restrict__ bias, int M, long N, long K,
+__global__ void __launch_bounds__(256, 8) int8_product_rows_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
+                                                                const float* __restrict__ sb, const float* __restrict__ bias, long N, long K,
                                                                 float* __restrict__ y) {
   __shared__ int part[8][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = warp % WARPS;
@@ -677,7 +763,6 @@ __global__ void __launch_bounds__(256) int8_product_rows_kernel(const int8_t* __
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int m = 0; m < ROWS; ++m) {
-          if (m >= M) break;
           const int4 x = __ldg(reinterpret_cast<const int4*>(a + m * K + k + u * kStep));
           sums[m] = __dp4a(v[u].x, x.x, __dp4a(v[u].y, x.y, __dp4a(v[u].z, x.z, __dp4a(v[u].w, x.w, sums[m]))));
         }
@@ -686,7 +771,6 @@ __global__ void __launch_bounds__(256) int8_product_rows_kernel(const int8_t* __
       const int4 v = __ldg(reinterpret_cast<const int4*>(w + k));
 #pragma unroll
       for (int m = 0; m < ROWS; ++m) {
-        if (m >= M) break;
         const int4 x = __ldg(reinterpret_cast<const int4*>(a + m * K + k));
         sums[m] = __dp4a(v.x, x.x, __dp4a(v.y, x.y, __dp4a(v.z, x.z, __dp4a(v.w, x.w, sums[m]))));
       }
@@ -708,21 +792,21 @@ __global__ void __launch_bounds__(256) int8_product_rows_kernel(const int8_t* __
   if (n >= N) return;
 #pragma unroll
   for (int m = 0; m < ROWS; ++m)
-    if (lane == m && m < M) {
+    if (lane == m) {
       const float v = (float)sums[m] * sa[m] * sb[n];
       y[m * N + n] = bias ? v + bias[n] : v;
     }
 }
 
 template <int ROWS>
-int product_rows(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K, float* y) {
+int product_rows(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long N, long K, float* y) {
   // as many warps for a channel as there are slices of 512 codes in its row, while the SMs are not full of warps
   const long full = (long)rt().sm_count * 32;
   const int warps = K > 2048 && N * 4 <= full ? 8 : K > 512 && N <= full ? 2 : 1;
   const unsigned grid = (unsigned)cgtb_ceil_div(N, 8 / warps);
-  if (warps == 8) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 8>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
-  else if (warps == 2) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 2>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
-  else CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 1>), grid, 256, 0, a, sa, b, sb, bias, (int)M, N, K, y);
+  if (warps == 8) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 8>), grid, 256, 0, a, sa, b, sb, bias, N, K, y);
+  else if (warps == 2) CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 2>), grid, 256, 0, a, sa, b, sb, bias, N, K, y);
+  else CGTB_LAUNCH((int8_product_rows_kernel<ROWS, 1>), grid, 256, 0, a, sa, b, sb, bias, N, K, y);
   CGTB_CHECK_LAUNCH("int8_product");
   return 0;
 }
@@ -752,8 +836,15 @@ CGTB_API int cgtb_int8_product(const int8_t* a, const float* sa, const int8_t* b
     CGTB_CHECK_LAUNCH("int8_product");
     return 0;
   }
-  if (M == 1) return product_rows<1>(a, sa, b, sb, bias, M, N, K, y);
-  if (M <= 4) return product_rows<4>(a, sa, b, sb, bias, M, N, K, y);
-  if (M <= 8) return product_rows<8>(a, sa, b, sb, bias, M, N, K, y);
+  // Measured at N = K = 4096, M = 1, 2, 4, 16, 32: a warp per channel 5.7, 6.9, 10.4 us; 16 channels and 8 rows a block 7.9, 8.0,
+  // 8.0, 8.5, 13.3 us; tcgen05 8.9 us. N = K = 1024, M = 32, 128, 256, 512: 16 x 8 a block 2.6, 4.9, 7.4, 12.5 us, 32 x 32 3.8,
+  // 3.9, 5.0, 8.3 us, tcgen05 6.1, 6.8, 6.7, 6.8 us. 100000 rows, N = K = 64: 60 us or more against 17.
+  if (M == 1) return product_rows<1>(a, sa, b, sb, bias, N, K, y);
+  if (M == 2) return product_rows<2>(a, sa, b, sb, bias, N, K, y);
+  const double products = (double)M * N * K;
+  if (M <= 16 || (products <= 4e8 && M <= 1L << 18 && M * N <= 1L << 19 && N * K <= 1L << 22)) {
+    const bool larger = products > 1e8 && 2 * cgtb_ceil_div(M, 32) * cgtb_ceil_div(N, 32) >= rt().sm_count;
+    return larger ? product_small<2, 4, 2>(a, sa, b, sb, bias, M, N, K, y) : product_small<1, 1, 2>(a, sa, b, sb, bias, M, N, K, y);
+  }
   return product_tc(a, sa, b, sb, bias, M, N, K, y);
 }
