@@ -133,18 +133,20 @@ __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)
         if (row0 + 8 * i < nrows) *reinterpret_cast<float4*>(dst + 8 * i * p.N) = finished(v[i], s, b, bias);
     }
   } else {
-    const int c = lane & 15;
+    const int c = lane & 15, row0 = lane >> 4;
     if (n0 + c < p.N) {
       const float s = columns[c], b = columns[256 + c];
-      float* dst = p.y + (m0 + (lane >> 4)) * p.N + n0 + c;
-#pragma unroll 4
-      for (int row = lane >> 4; row < nrows; row += 2, dst += 2 * p.N) {
-        const float v = block[block_at(row, c >> 2) + (c & 3)];
-        *dst = bias ? v * s + b : v * s;
-      }
+      float* dst = p.y + (m0 + row0) * p.N + n0 + c;
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = block[block_at(row0 + 2 * i, c >> 2) + (c & 3)];
+#pragma unroll
+      for (int i = 0; i < 16; ++i, dst += 2 * p.N)
+        if (row0 + 2 * i < nrows) *dst = bias ? v[i] * s + b : v[i] * s;
     }
   }
 }
+
 // A warp's share of a tile: its 32 rows, every other chunk of 16 columns. The next chunk is on its way from TMEM meanwhile;
 // release() is called when nothing more is read there.
 template <typename F>
