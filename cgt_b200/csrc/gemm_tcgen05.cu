@@ -498,7 +498,7 @@ int sgemm_tc_check() {
     int code = *g_err_host;
     *g_err_host = 0;
     return fail("a bounded device-side wait expired (code %d: 3-7 a barrier of the tensor-core GEMM / convolution kernels, 8 a rank "
-                "of the peer-memory all-reduce did not arrive); the result of that call is invalid", code);
+                "of the peer-memory all-reduce did not arrive, 9 a copy of layer norm's gradients); the result of that call is invalid", code);
   }
   return 0;
 }

@@ -1,6 +1,7 @@
 // Layer norm with its gradients, dropout from a counter-based generator, and rows in 8-bit integers with a scale each, for
 // sm_100a.
 #include "runtime.h"
+#include "tc_util.h"
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -178,16 +179,43 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 // memory (no other thread touches them: no barrier): registers could hold one row more at most.
 constexpr int kAhead = 2;
 template <typename T, int VEC, int N, int TEAM>
-constexpr size_t norm_backward_bytes() { return (size_t)(kAhead + 1) * 2 * N * team_block<TEAM>() * VEC * sizeof(T); }
+constexpr size_t norm_backward_array() { return (size_t)N * team_block<TEAM>() * VEC * sizeof(T) + (VEC == 1 ? 32 : 0); }   // of one stage
+template <typename T, int VEC, int N, int TEAM>
+constexpr size_t norm_backward_bytes() { return (kAhead + 1) * 2 * norm_backward_array<T, VEC, N, TEAM>(); }
+
+// VEC 1, for rows that start anywhere among others. Element by element, the copies above are four bytes each and bound the kernel
+// (16384 x 2047: 111 us, now 68 us). But the rows that a block's teams take in one step lie one behind the other, so one thread
+// brings all of them by a bulk copy, from the 16-byte boundary before the first to the one behind the last. Where that would
+// leave the array, at its two ends, the rows are loaded directly.
+template <typename T>
+struct Span {
+  const unsigned char* from;     // on a 16-byte boundary
+  uint32_t bytes, shift;         // `shift`: of the first element
+  bool inside;
+  __device__ __forceinline__ Span(const T* array, long size, long first, long count) {
+    const uintptr_t begin = (uintptr_t)array, lo = begin + first * sizeof(T), hi = lo + count * sizeof(T);
+    const uintptr_t lo16 = lo & ~(uintptr_t)15, hi16 = (hi + 15) & ~(uintptr_t)15;
+    from = (const unsigned char*)lo16;
+    bytes = (uint32_t)(hi16 - lo16);
+    shift = (uint32_t)(lo - lo16);
+    inside = lo16 >= begin && hi16 <= begin + size * sizeof(T);
+  }
+};
+__device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
 
 template <typename T, int VEC, int N, int TEAM, bool ONE>
 __global__ void __launch_bounds__(team_block<TEAM>(), (TEAM == 1024 || VEC * N * sizeof(T) == 32 && sizeof(T) == 4 ? 1024 : 512) / team_block<TEAM>())
 norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy, long R, int C, T eps, T* __restrict__ dx,
-                     T* __restrict__ part, T* __restrict__ dgain, T* __restrict__ dbias) {
+                     T* __restrict__ part, T* __restrict__ dgain, T* __restrict__ dbias, int* err) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
   typedef Pack<T, VEC> P;
   extern __shared__ __align__(16) unsigned char ahead_raw[];
   __shared__ __align__(16) T sums[2 * (kBlock / 32) * 2];
+  __shared__ __align__(8) uint64_t full[kAhead + 1];
+  constexpr size_t kArray = norm_backward_array<T, VEC, N, TEAM>();
   P* ahead = reinterpret_cast<P*>(ahead_raw) + threadIdx.x;     // [kAhead + 1][x, gy][N][thread]
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   const long step = (long)gridDim.x * kTeams;
@@ -195,43 +223,88 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     inside[i] = (i * TEAM + t) * VEC < C;
-    if (!inside[i])      // never written again: columns beyond C are zeros in every row
+    if (VEC > 1 && !inside[i])      // never written again: columns beyond C are zeros in every row
       for (int k = 0; k < 2 * (kAhead + 1); ++k)
         for (int j = 0; j < VEC; ++j) ahead[(k * N + i) * kBlock].v[j] = T(0);
   }
+  if (VEC == 1 && threadIdx.x == 0) {
+    for (int i = 0; i <= kAhead; ++i) tc::mbar_init(tc::smem_u32(&full[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (VEC == 1) __syncthreads();
+  // r: this team's row; VEC 1: the first team's, by one thread for all
   auto fetch = [&](int stage, long r) {
-    if (r < R) {
-      const T *from_x = x + r * C + t * VEC, *from_g = gy + r * C + t * VEC;
-      P* to = ahead + stage * (2 * N * kBlock);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (inside[i]) {
-          copy_async<sizeof(P)>(to + i * kBlock, from_x + i * TEAM * VEC);
-          copy_async<sizeof(P)>(to + (N + i) * kBlock, from_g + i * TEAM * VEC);
+    if constexpr (VEC == 1) {
+      if (threadIdx.x == 0 && r < R) {
+        const long rows = R - r < kTeams ? R - r : kTeams;
+        const Span<T> sx(x, R * C, r * C, rows * C), sg(gy, R * C, r * C, rows * C);
+        if (sx.inside && sg.inside) {
+          const uint32_t bar = tc::smem_u32(&full[stage]);
+          tc::mbar_arrive_expect_tx(bar, sx.bytes + sg.bytes);
+          copy_bulk(ahead_raw + (stage * 2) * kArray, sx.from, sx.bytes, bar);
+          copy_bulk(ahead_raw + (stage * 2 + 1) * kArray, sg.from, sg.bytes, bar);
         }
+      }
+    } else {
+      if (r < R) {
+        const T *from_x = x + r * C + t * VEC, *from_g = gy + r * C + t * VEC;
+        P* to = ahead + stage * (2 * N * kBlock);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (inside[i]) {
+            copy_async<sizeof(P)>(to + i * kBlock, from_x + i * TEAM * VEC);
+            copy_async<sizeof(P)>(to + (N + i) * kBlock, from_g + i * TEAM * VEC);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   long r = (long)blockIdx.x * kTeams + team;
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) fetch(i, r + i * step);
+  for (int i = 0; i < kAhead; ++i) fetch(i, (VEC == 1 ? (long)blockIdx.x * kTeams : r) + i * step);
   Row<T, VEC, N, TEAM> w, dg, db;
   w.load(gain, C, t, T(0));
 #pragma unroll
   for (int e = 0; e < E; ++e) dg.v[e] = db.v[e] = T(0);
   int stage = 0;
+  uint32_t phases = 0;       // of the stages' barriers
   for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
-    fetch(stage >= 1 ? stage - 1 : kAhead, r + kAhead * step);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+    // VEC 1: the stage that is filled now was read in the step before; teams of several warps met at a barrier since
+    if (VEC == 1 && TEAM <= 32) __syncthreads();
+    fetch(stage >= 1 ? stage - 1 : kAhead, (VEC == 1 ? first : r) + kAhead * step);
     Row<T, VEC, N, TEAM> a, g;
-    const P* from = ahead + stage * (2 * N * kBlock);
+    if constexpr (VEC == 1) {
+      const long rows = R - first < kTeams ? R - first : kTeams;
+      const Span<T> sx(x, R * C, first * C, rows * C), sg(gy, R * C, first * C, rows * C);
+      if (sx.inside && sg.inside) {
+        if (!tc::mbar_wait(tc::smem_u32(&full[stage]), (phases >> stage) & 1u)) {     // bounded; the sums are invalid then
+          *(volatile int*)err = 9;
+          __threadfence_system();
+        }
+        phases ^= 1u << stage;
+        const T* from_x = reinterpret_cast<const T*>(ahead_raw + (stage * 2) * kArray + sx.shift) + team * C + t;
+        const T* from_g = reinterpret_cast<const T*>(ahead_raw + (stage * 2 + 1) * kArray + sg.shift) + team * C + t;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const P px = from[i * kBlock], pg = from[(N + i) * kBlock];
+        for (int i = 0; i < N; ++i) {
+          a.v[i] = inside[i] ? from_x[i * TEAM] : T(0);
+          g.v[i] = inside[i] ? from_g[i * TEAM] : T(0);
+        }
+      } else {
+        const int valid = r < R ? C : 0;
+        a.load(x + r * C, valid, t, T(0));
+        g.load(gy + r * C, valid, t, T(0));
+      }
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+      const P* from = ahead + stage * (2 * N * kBlock);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        a.v[i * VEC + j] = px.v[j];
-        g.v[i * VEC + j] = pg.v[j];
+      for (int i = 0; i < N; ++i) {
+        const P px = from[i * kBlock], pg = from[(N + i) * kBlock];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          a.v[i * VEC + j] = px.v[j];
+          g.v[i * VEC + j] = pg.v[j];
+        }
       }
     }
     if (++stage > kAhead) stage = 0;
@@ -542,12 +615,12 @@ bool with_team(long C, F f) {
   else if (C <= 32L * E) f(std::integral_constant<int, 32>());
   else if (C <= 64L * E) f(std::integral_constant<int, 64>());
   else if (C <= 128L * E) f(std::integral_constant<int, 128>());
-  else if constexpr (kMaxTeam >= 1024) {
-    if (C <= 256L * E) f(std::integral_constant<int, 256>());
-    else if (C <= 512L * E) f(std::integral_constant<int, 512>());
-    else if (C <= 1024L * E) f(std::integral_constant<int, 1024>());
-    else return false;
-  } else return false;
+  else {
+    if constexpr (kMaxTeam >= 256) { if (C <= 256L * E) { f(std::integral_constant<int, 256>()); return true; } }
+    if constexpr (kMaxTeam >= 512) { if (C <= 512L * E) { f(std::integral_constant<int, 512>()); return true; } }
+    if constexpr (kMaxTeam >= 1024) { if (C <= 1024L * E) { f(std::integral_constant<int, 1024>()); return true; } }
+    return false;
+  }
   return true;
 }
 
@@ -592,9 +665,9 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
 // The gradients by teams of E elements a thread; dgain and dbias are complete, or in `part` for P blocks. 1: failed, -1: no team
 // is that large
 template <typename T, int E, int kMaxTeam>
-int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias, T*& part, long& P) {
-  const bool wide = starts_on_16<T>(C, {x, gain, gy, dx});
-  int failed = 0;
+int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, bool wide, T* dx, T* dgain, T* dbias, T*& part, long& P) {
+  int failed = 0, *const err = tc_error_flag();
+  if (!err) return 1;
   const bool held = with_team<E, kMaxTeam>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
     auto launch = [&](auto width) {
@@ -615,7 +688,7 @@ int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, 
         config.stream = rt().stream;
         config.attrs = &attr;
         config.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias);
+        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias, err);
         if (e != cudaSuccess) failed = fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e));
         g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
         return;
@@ -625,7 +698,7 @@ int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, 
       P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
       part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
       if (!part) failed = 1;
-      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr);
+      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, err);
     };
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
     else launch(std::integral_constant<int, 1>());
@@ -637,12 +710,15 @@ template <typename T>
 int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias) {
   T* part = nullptr;
   long P = 0;
-  // 16 elements a thread save steps of the sums (float32, 30000 x 784: 72 us with 8, 48 us with 16); with teams of more than four
-  // warps too few rows are under way at a time (8192 x 4096: 79 us with 8, 85 us with 16), with float64 registers run out
-  // (8192 x 1024: 46 us with 4, 51 us with 8)
+  // 64 bytes of a row a thread save steps of the sums (float32, 30000 x 784: 72 us with 32, 48 us with 64; float64, 4000 x 2047: 51
+  // and 38 us), 32 bytes where a row has not enough for that, or is short and float64 (100000 x 64: 29 against 33 us). Arrays
+  // that start on 16-byte boundaries are read 16 bytes at a time (100000 x 64: 20 against 31 us, 4000 x 5000: 53 against 66 us),
+  // but in between, where two or four rows are under way on an SM, by the bulk copies all the same (8192 x 4096: 69 against 86 us).
+  const bool starts = starts_on_16<T>(C, {x, gain, gy, dx});
+  const bool wide = starts && (sizeof(T) == 8 ? C <= 1024 : C <= 1024 || C > 4096);
   int failed;
-  if (sizeof(T) == 4 && C > 16 && C <= 2048) failed = norm_backward_teams<T, 16, 128>(x, gain, gy, R, C, eps, dx, dgain, dbias, part, P);
-  else failed = norm_backward_teams<T, 32 / sizeof(T), 1024>(x, gain, gy, R, C, eps, dx, dgain, dbias, part, P);
+  if (C <= 16 || (sizeof(T) == 8 && wide)) failed = norm_backward_teams<T, 32 / sizeof(T), 256>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
+  else failed = norm_backward_teams<T, 64 / sizeof(T), 512>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
   if (failed > 0) return 1;
   if (failed < 0 && C <= kLongThreads * wide_elements<T>()) {
     auto launch = [&](auto width) {
@@ -652,7 +728,7 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
       part = (T*)scratch((size_t)P * 2 * C * sizeof(T));
       if (part) CGTB_LAUNCH(kernel, (unsigned)P, kLongThreads, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part);
     };
-    if (starts_on_16<T>(C, {x, gain, gy, dx})) launch(std::integral_constant<int, 16 / sizeof(T)>());
+    if (starts) launch(std::integral_constant<int, 16 / sizeof(T)>());
     else launch(std::integral_constant<int, 1>());
     if (!part) return 1;
   } else if (failed < 0) {
