@@ -642,13 +642,14 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   const bool wide = starts_on_16<T>(C, {x, gain, bias, y});
   const bool held = with_team<E, 1024>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
-    auto launch = [&](auto width) {
-      constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, E / decltype(width)::value, TEAM>;
+    auto launch = [&](auto width, auto elements) {
+      constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, decltype(elements)::value / decltype(width)::value, TEAM>;
       const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
       CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y);
     };
-    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
-    else launch(std::integral_constant<int, 1>());
+    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>(), std::integral_constant<int, E>());
+    else if (TEAM > 1 && C <= TEAM * (E * 3 / 4)) launch(std::integral_constant<int, 1>(), std::integral_constant<int, E * 3 / 4>());     // fewer places without an element
+    else launch(std::integral_constant<int, 1>(), std::integral_constant<int, E>());
   });
   if (!held && C <= kLongThreads * wide_elements<T>()) {
     const unsigned grid = (unsigned)std::min<long>(R, rt().sm_count);
@@ -675,7 +676,7 @@ int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, 
       constexpr size_t bytes = norm_backward_bytes<T, VEC, E / VEC, TEAM>();
       constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM, false>, one = norm_backward_kernel<T, VEC, E / VEC, TEAM, true>;
       const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
-      if (steps <= 32) {      // a cluster of eight blocks makes up to four steps each: less than another kernel takes
+      if (steps <= 8) {       // (512 x 256, 32 steps: 7.0 us by eight blocks, 5.1 us by more and another kernel)
         (void)resident_blocks<one, kBlock, bytes>();      // allows the shared memory
         cudaLaunchAttribute attr = {};
         attr.id = cudaLaunchAttributeClusterDimension;
@@ -877,21 +878,32 @@ __device__ __forceinline__ uint32_t team_max(uint32_t m, uint32_t* part, int tur
   return m;
 }
 
-// A team holds a row, like layer norm's; the next row's loads are under way meanwhile. Bound by the bytes of x.
-template <int VEC, int N, int TEAM>
+// A team holds a row, four consecutive elements of it in a thread at a time, whose codes are one word; rows that do not start on
+// 16-byte boundaries are loaded element by element (the four loads of a warp touch the same lines: 500000 x 17 15.5 us, with
+// consecutive elements in consecutive threads and stores of single bytes 38 us). The next row's loads are under way meanwhile.
+// Bound by the bytes of x.
+template <bool WIDE, int N, int TEAM>
 __global__ void __launch_bounds__(team_block<TEAM>()) quantize_rows_kernel(const float* __restrict__ x, long R, int C, int Cp, int8_t* __restrict__ codes,
                                                                            float* __restrict__ scales) {
-  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = 4 * N;
   __shared__ uint32_t part[2 * (kBlock / 32)];
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   const long step = (long)gridDim.x * kTeams;
   long r = (long)blockIdx.x * kTeams + team;
-  Row<float, VEC, N, TEAM> row, next;
-  if (r < R) next.load(x + r * C, C, t, 0.f);
+  Row<float, 4, N, TEAM> row, next;
+  auto load = [&](long at) {
+    if constexpr (WIDE) next.load(x + at * C, C, t, 0.f);
+    else {
+      const float* from = x + at * C + 4 * t;
+#pragma unroll
+      for (int e = 0; e < E; ++e) next.v[e] = (e / 4 * TEAM + t) * 4 + e % 4 < C ? from[e / 4 * TEAM * 4 + e % 4] : 0.f;
+    }
+  };
+  if (r < R) load(r);
   int turn = 0;
   for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step, turn ^= 1) {
     row = next;
-    if (r + step < R) next.load(x + (r + step) * C, C, t, 0.f);
+    if (r + step < R) load(r + step);
     uint32_t m = 0;   // as whole numbers the bits of |x| order like the values, infinities and NaN above all
 #pragma unroll
     for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(row.v[e]) & 0x7fffffffu);
@@ -900,25 +912,10 @@ __global__ void __launch_bounds__(team_block<TEAM>()) quantize_rows_kernel(const
       const bool some = m != 0 && m < 0x7f800000u;
       const float largest = __uint_as_float(m), inverse = 127.0f / largest;
       const bool exact = !(inverse <= 3.0e38f);      // rows of the smallest numbers
-      uint32_t w[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = some ? codes_of<VEC>(row.v + i * VEC, largest, inverse, exact) : 0u;
-      if constexpr (TEAM == 1 && VEC == 1 && N == 16) {     // the whole row is this thread's
-        uint4 all;
-        uint32_t* q = &all.x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q[i] = __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0040), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0040), 0x5410);
-        *reinterpret_cast<uint4*>(codes + r * Cp) = all;
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = (i * TEAM + t) * VEC;
-          if (c < Cp) {
-            if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(codes + r * Cp + c) = w[i];
-            else codes[r * Cp + c] = (int8_t)w[i];
-          }
-        }
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * TEAM + t) * 4;
+        if (c < Cp) *reinterpret_cast<uint32_t*>(codes + r * Cp + c) = some ? codes_of<4>(row.v + i * 4, largest, inverse, exact) : 0u;
       }
       if (t == 0) scales[r] = scale_of(m);
     }
@@ -990,15 +987,15 @@ CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, f
   if (R == 0) return 0;
   const long Cp = cgtb_ceil_div(C, 16) * 16;
   const bool wide = starts_on_16<float>(C, {x});
-  auto launch = [&](auto width, auto elements, auto team) {
-    constexpr int VEC = decltype(width)::value, TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
-    constexpr auto kernel = quantize_rows_kernel<VEC, decltype(elements)::value / VEC, TEAM>;
+  auto launch = [&](auto wide16, auto elements, auto team) {
+    constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
+    constexpr auto kernel = quantize_rows_kernel<decltype(wide16)::value, decltype(elements)::value / 4, TEAM>;
     const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
     CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, R, (int)C, (int)Cp, codes, scales);
   };
   auto either = [&](auto elements, auto team) {
-    if (wide) launch(std::integral_constant<int, 4>(), elements, team);
-    else launch(std::integral_constant<int, 1>(), elements, team);
+    if (wide) launch(std::true_type(), elements, team);
+    else launch(std::false_type(), elements, team);
   };
   bool held = with_team<16, 1024>(Cp, [&](auto team) { either(std::integral_constant<int, 16>(), team); });
   if (!held && Cp <= 1024 * 20) {
