@@ -486,6 +486,8 @@ static uint64_t span_key(cgtbInterp* it, const Span& s) {
     if (in.klass != kDevice) continue;
     for (auto& r : in.reads) h = key_of_object(h, get(it, r), r.dev);
     h = key_of_object(h, get(it, in.write), in.write.dev);
+    // a workspace that has grown for other extents since is at another place
+    h = mix(mix(h, (uint64_t)(uintptr_t)in.scratch.ptr), (uint64_t)(uintptr_t)in.scratch.outer_ptr);
   }
   if (s.collects) {
     h = mix(h, (uint64_t)(uintptr_t)it->out_stage);
@@ -947,6 +949,7 @@ static int run_span(cgtbInterp* it, Span& s) {
   long l0 = g_kernel_launches.load();
   if (issue_device(it, s, profile, false)) return 1;
   mark_device_fired(it, s);
+  if (use_graphs) s.last_key = span_key(it, s);   // with the workspaces that this run has made
   it->last_launches += g_kernel_launches.load() - l0;
   return 0;
 }

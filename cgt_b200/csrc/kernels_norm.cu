@@ -984,6 +984,7 @@ CGTB_API int cgtb_dropout(int dtype, const void* x, long n, double p, const int6
 CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, float* scales) {
   if (!require_runtime("cgtb_quantize_rows")) return 1;
   if (R < 0 || C < 0) return fail("cgtb_quantize_rows: negative extent");
+  if ((uintptr_t)codes & 15) return fail("cgtb_quantize_rows: the codes have to start on a 16-byte boundary");
   if (R == 0) return 0;
   const long Cp = cgtb_ceil_div(C, 16) * 16;
   const bool wide = starts_on_16<float>(C, {x});

@@ -290,7 +290,7 @@ def test_refused_calls_leave_the_library_usable(rt):
         ("cgtb_dropout", (11, d.ptr, 32, -0.1, state.ptr, 0, d.ptr)),
         ("cgtb_dropout", (5, d.ptr, 32, 0.1, state.ptr, 0, d.ptr)),
         ("cgtb_dropout", (11, d.ptr, -32, 0.1, state.ptr, 0, d.ptr)),
-        ("cgtb_quantize_rows", (d.ptr, -1, 32, c.ptr, s.ptr)),
+        ("cgtb_quantize_rows", (d.ptr, -1, 32, c.ptr, s.ptr)), ("cgtb_quantize_rows", (d.ptr, 1, 16, off, s.ptr)),
         ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, 4, 4, 24, d.ptr)),
         ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, 4, 4, 131072, d.ptr)),
         ("cgtb_int8_product", (c.ptr, s.ptr, c.ptr, s.ptr, None, -4, 4, 32, d.ptr)),
@@ -470,3 +470,25 @@ def test_arrays_of_other_ranks(rt):
     for (got, x) in ((ya, v[None]), (yb, t.reshape(-1, 24))):
         assert (np.abs(got.reshape(x.shape) - ref.norm(x, gain, bias, 1e-5)[0]) <= ref.norm_bounds(x, gain, bias, None, 1e-5)).all()
     assert np.array_equal(d, ref.dropout(t, 0.5, 1, 0, 0))
+
+
+def test_a_workspace_that_grew_is_not_replayed_at_its_old_place(rt):
+    """A function with an open batch goes back to a shape whose captured graph used a smaller workspace: the graph is not
+    launched again before it is captured anew, and all results are right."""
+    with cgt.scoped_update_config(specialise_shapes=False):
+        x, gain, bias = cgt.matrix("x", fixed_shape=(None, 300)), _shared(np.ones(300, "f4")), _shared(np.zeros(300, "f4"))
+        y = nn.layer_norm(x, gain, bias)
+        grads = core.pullback([y], [y * 2.0], [gain, bias])
+        f = cgt.function([x], grads)
+    wants = {}
+    launches = []
+    for rows in (400, 400, 400, 400, 9000, 400, 9000, 9000, 9000, 400, 400, 400, 400):
+        v = np.random.RandomState(rows).randn(rows, 300).astype("f4")
+        if rows not in wants:
+            g = 2 * ref.norm(v, np.ones(300, "f4"), np.zeros(300, "f4"), 1e-5)[0]
+            wants[rows] = [w for w in ref.norm_gradients(v, np.ones(300, "f4"), g, 1e-5)[1:]]
+        for (got, want) in zip(f(v), wants[rows]):
+            # sums of up to 9000 terms of either sign, each off by a few roundings
+            np.testing.assert_allclose(got, want, rtol=1e-4, atol=9000 * 8 * 2.0 ** -24)
+        launches.append(f.stats()["last_graph_launches"])
+    assert launches[3] == 1 and launches[5] == 0 and launches[-1] == 1
