@@ -200,3 +200,24 @@ def test_an_extent_that_is_computed_from_an_open_one():
     for shape in ((3, 20), (5, 16), (2, 1)):
         v = np.random.RandomState(0).randn(*shape).astype("f4")
         assert all(np.array_equal(a, b) for (a, b) in zip(run(v), ref.quantize(v)))
+
+
+def test_a_checkpoint_holds_the_streams_state():
+    x = cgt.matrix("x", fixed_shape=(4, 4))
+    stream, norm = nn.RandomStream(3), nn.LayerNorm(4)
+    loss = cgt.square(nn.dropout(norm(x), 0.5, stream)).sum()
+    updates = nn.sgd(loss, nn.get_parameters(loss), 0.1) + stream.updates()
+    held = cgt.state_variables(updates, [loss], nn.get_parameters(loss))
+    assert stream.state in held and norm.gain in held and norm.bias in held and len(nn.get_parameters(loss)) == 2
+
+
+def test_layers_parameters():
+    layer = nn.LayerNorm(6, name="n")
+    assert np.array_equal(layer.gain.op.get_value(), np.ones(6)) and np.array_equal(layer.bias.op.get_value(), np.zeros(6))
+    np.random.seed(0)
+    affine = nn.Affine(5, 3, weight_init=nn.XavierNormal(), bias_init=nn.IIDGaussian())
+    q = nn.Int8Affine(affine)
+    codes, scales = ref.quantize(affine.weight.op.get_value().T.copy())
+    assert np.array_equal(q.codes.op.get_value(), codes) and np.array_equal(q.scales.op.get_value(), scales)
+    assert np.array_equal(q.bias.op.get_value(), affine.bias.op.get_value()[0]) and q.codes.op.get_value().dtype == np.int8
+    assert not nn.get_parameters(q(cgt.matrix("x")).sum())       # nothing to train

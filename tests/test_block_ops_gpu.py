@@ -492,3 +492,78 @@ def test_a_workspace_that_grew_is_not_replayed_at_its_old_place(rt):
             np.testing.assert_allclose(got, want, rtol=1e-4, atol=9000 * 8 * 2.0 ** -24)
         launches.append(f.stats()["last_graph_launches"])
     assert launches[3] == 1 and launches[5] == 0 and launches[-1] == 1
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("R,C", [(9, 64), (40, 17), (5, 1001), (3, 9000)])
+def test_quantize_rows_that_start_anywhere(rt, R, C, offset):
+    x = _norm_inputs(R, C, "f4")[0]
+    d = Dev(np.concatenate([np.zeros(offset, "f4"), x.reshape(-1), np.full(4, np.inf, "f4")]))
+    Cp = -(-C // 16) * 16
+    codes, scales = Dev(np.full(R * Cp + 16, 99, "i1")), Dev(np.full(R + 1, 7, "f4"))
+    call("cgtb_quantize_rows", ctypes.c_void_p(d.w.data + 4 * offset), R, C, codes.ptr, scales.ptr)
+    want = ref.quantize(x)
+    flat = codes.get()
+    assert np.array_equal(flat[:R * Cp].reshape(R, Cp), want[0]) and (flat[R * Cp:] == 99).all()
+    assert np.array_equal(scales.get()[:R], want[1]) and scales.get()[R] == 7
+
+
+@pytest.mark.parametrize("M,N", [(1, 33), (5, 20), (40, 50), (300, 129), (700, 257)])
+def test_int8_product_writes_its_result_and_nothing_else(rt, M, N):
+    """Results, scales and biases that start on any element; what lies around the result stays."""
+    rs = np.random.RandomState(M)
+    K = 144
+    a, b = rs.randint(-128, 128, (M, K)).astype("i1"), rs.randint(-128, 128, (N, K)).astype("i1")
+    sa, sb, bias = rs.rand(M).astype("f4"), rs.rand(N).astype("f4"), rs.randn(N).astype("f4")
+    want, bound = ref.product(a, sa, b, sb, bias)
+
+    def shifted(v, k):
+        d = Dev(np.concatenate([np.zeros(k, "f4"), v]))
+        return d, ctypes.c_void_p(d.w.data + 4 * k)
+    (ka, pa), (kb, pb), (kc, pc) = shifted(sa, 1), shifted(sb, 3), shifted(bias, 2)
+    da, db = Dev(a), Dev(b)
+    for offset in (0, 1, 2):
+        y = Dev(np.full(M * N + 8, 7, "f4"))
+        call("cgtb_int8_product", da.ptr, pa, db.ptr, pb, pc, M, N, K, ctypes.c_void_p(y.w.data + 4 * offset))
+        flat = y.get()
+        assert (np.abs(flat[offset:offset + M * N].reshape(M, N) - want) <= bound).all()
+        assert (flat[:offset] == 7).all() and (flat[offset + M * N:] == 7).all()
+
+
+def test_gradients_of_a_norm_that_is_used_twice(rt):
+    """One layer's gain and bias in two places: their gradients are the sums of both, in a step that is replayed."""
+    rs = np.random.RandomState(2)
+    R, C = 30, 77
+    layer = nn.LayerNorm(C)
+    layer.gain.op.set_value((1 + 0.2 * rs.randn(C)).astype("f4"))
+    layer.bias.op.set_value(rs.randn(C).astype("f4"))
+    x, t = cgt.matrix("x", fixed_shape=(R, C)), cgt.matrix("t", fixed_shape=(R, C))
+    y = layer(cgt.tanh(layer(x)))
+    loss = (y * t).sum()
+    f = cgt.function([x, t], cgt.grad(loss, [layer.gain, layer.bias]))
+    gain, bias = layer.gain.op.get_value().astype("f8"), layer.bias.op.get_value().astype("f8")
+    for _ in range(4):
+        xv, tv = rs.randn(R, C).astype("f4"), rs.randn(R, C).astype("f4")
+        h1 = np.tanh(ref.norm(xv.astype("f8"), gain, bias, 1e-5)[0]).astype("f8")
+        d2, g2, b2 = ref.norm_gradients(h1, gain, tv.astype("f8"), 1e-5)
+        _d, g1, b1 = ref.norm_gradients(xv.astype("f8"), gain, (d2 * (1 - h1 * h1)).astype("f8"), 1e-5)
+        for (got, want) in zip(f(xv, tv), (g1 + g2, b1 + b2)):
+            # sums of 60 terms of order one, each through some thirty float32 roundings
+            np.testing.assert_allclose(got, want.astype("f8"), atol=60 * 30 * 2.0 ** -24 * 3)
+
+
+def test_one_variable_for_every_operand(rt):
+    """The gradient of a leaf that is the row, the gain and the bias at once is the sum of the three."""
+    v = (np.random.RandomState(0).rand(50) + 0.5).astype("f4")
+    x = _shared(v)
+    y = nn.layer_norm(x, x, x)
+    f = cgt.function([], [y] + core.pullback([y], [x], [x]))
+    want = ref.norm(v[None], v, v, 1e-5)[0][0]
+    dx, dg, db = ref.norm_gradients(v[None], v, v[None], 1e-5)
+    by, bx, bg, bb = ref.norm_bounds(v[None], v, v, v[None], 1e-5)
+    # the two additions that join the three gradients round once each
+    joined = bx[0] + bg + bb + 2 * ref.U["f4"] * (np.abs(dx[0]) + np.abs(dg) + np.abs(db))
+    for _ in range(3):
+        got = f()
+        assert (np.abs(got[0] - want) <= by[0]).all()
+        assert (np.abs(got[1] - (dx[0] + dg + db)) <= joined).all()
