@@ -657,32 +657,39 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
 
 // ------------------------------------------------------------------------------------------------
 // Small products and few rows, where the kernels above spend most of their time on beginning (5 to 8 us whatever they do). A
-// block makes 16 CT output channels x 8 NT rows; its eight warps take turns with 64 codes of K, UNROLL such steps in flight, and
-// join their sums in shared memory at the end. The weights are the matrix instructions' A operand (16 channels), the rows their
+// block makes 16 CT output channels x 8 NT TW rows; its eight warps, TW of them beside each other, take turns with 64 codes of K,
+// UNROLL such steps in flight, and join their sums in shared memory at the end. The weights are the matrix instructions' A operand (16 channels), the rows their
 // B operand (8 rows): with few rows nothing is multiplied in vain. No shared memory in the loop: which codes of K an instruction
 // sees in which of its places is free as long as both operands agree, so a thread loads 16 consecutive codes of a row and gives
-// them to two instructions as they are. Bound by latency, or by the bytes of the weights: 128 x 256 x 784 2.5 us,
-// 8 x 4096 x 4096 8.0 us (2.1 TB/s).
+// them to two instructions as they are, and rows that start on any 16 bytes cost little (the TMA loads above take a quarter longer
+// where K is an odd multiple of 16). Bound by latency, then by what the blocks read again from L2: 128 x 256 x 784 2.4 us,
+// 500 x 1001 x 1008 6.5 us (tcgen05 8.7), 8 x 4096 x 4096 8 us (2.1 TB/s).
 // ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int CT, int NT, int UNROLL>
+template <int CT, int NT, int TW>
+struct Small {
+  static constexpr int kChannels = 16 * CT, kTokens = 8 * NT * TW, kSlices = 8 / TW;
+  static constexpr int kPitch = kChannels + 4;   // the stores of a warp, 8 channels of 4 tokens two apart, reach all banks
+  static constexpr int kBytes = kSlices * kTokens * kPitch * 4;
+};
+template <int CT, int NT, int TW, int UNROLL>
 __global__ void __launch_bounds__(256) int8_product_small_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa, const int8_t* __restrict__ b,
                                                                  const float* __restrict__ sb, const float* __restrict__ bias, long M, long N, long K,
                                                                  float* __restrict__ y) {
-  constexpr int kChannels = 16 * CT, kTokens = 8 * NT, kPitch = kChannels + 1;
-  __shared__ int joined[8][kTokens * kPitch];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long n0 = (long)blockIdx.x * kChannels, m0 = (long)blockIdx.y * kTokens;
+  using S = Small<CT, NT, TW>;
+  extern __shared__ int joined[];         // [slice][token][channel]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, slice = warp / TW, token0 = warp % TW * (8 * NT);
+  const long n0 = (long)blockIdx.x * S::kChannels, m0 = (long)blockIdx.y * S::kTokens;
   // rows beyond the operands are read as the last one: their results are not stored
   const int8_t *w[2 * CT], *x[NT];
 #pragma unroll
   for (int i = 0; i < 2 * CT; ++i) w[i] = b + (n0 + g + 8 * i < N ? n0 + g + 8 * i : N - 1) * K + t * 16;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) x[j] = a + (m0 + g + 8 * j < M ? m0 + g + 8 * j : M - 1) * K + t * 16;
+  for (int j = 0; j < NT; ++j) x[j] = a + (m0 + token0 + g + 8 * j < M ? m0 + token0 + g + 8 * j : M - 1) * K + t * 16;
   int c[CT][NT][4];
 #pragma unroll
   for (int i = 0; i < CT; ++i)
@@ -691,15 +698,16 @@ __global__ void __launch_bounds__(256) int8_product_small_kernel(const int8_t* _
 #pragma unroll
       for (int k = 0; k < 4; ++k) c[i][j][k] = 0;
   const long last = K - t * 16;      // this thread's codes of a step are there for k < last
-  for (long k = warp * 64; k < K; k += 512 * UNROLL) {
+  constexpr int kStep = S::kSlices * 64;
+  for (long k = slice * 64; k < K; k += kStep * UNROLL) {
     uint4 wv[UNROLL][2 * CT], xv[UNROLL][NT];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const bool there = k + u * 512 < last;
+      const bool there = k + u * kStep < last;
 #pragma unroll
-      for (int i = 0; i < 2 * CT; ++i) wv[u][i] = there ? __ldg(reinterpret_cast<const uint4*>(w[i] + k + u * 512)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 2 * CT; ++i) wv[u][i] = there ? __ldg(reinterpret_cast<const uint4*>(w[i] + k + u * kStep)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) xv[u][j] = there ? __ldg(reinterpret_cast<const uint4*>(x[j] + k + u * 512)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < NT; ++j) xv[u][j] = there ? __ldg(reinterpret_cast<const uint4*>(x[j] + k + u * kStep)) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
@@ -711,31 +719,42 @@ __global__ void __launch_bounds__(256) int8_product_small_kernel(const int8_t* _
           mma_16832(c[i][j], wv[u][2 * i].z, wv[u][2 * i + 1].z, wv[u][2 * i].w, wv[u][2 * i + 1].w, xv[u][j].z, xv[u][j].w);
         }
   }
+  int* own = joined + (slice * S::kTokens + token0) * S::kPitch;
 #pragma unroll
   for (int i = 0; i < CT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) joined[warp][(8 * j + 2 * t + (k & 1)) * kPitch + 16 * i + 8 * (k >> 1) + g] = c[i][j][k];
+      for (int k = 0; k < 4; ++k) own[(8 * j + 2 * t + (k & 1)) * S::kPitch + 16 * i + 8 * (k >> 1) + g] = c[i][j][k];
   __syncthreads();
-  const int channel = threadIdx.x % kChannels;
+  const int channel = threadIdx.x % S::kChannels;
   const long n = n0 + channel;
   if (n < N) {
     const float s = sb[n], shift = bias ? bias[n] : 0.f;
-    for (int token = threadIdx.x / kChannels; token < kTokens && m0 + token < M; token += 256 / kChannels) {
+    constexpr int kRowsAtOnce = 256 / S::kChannels;
+#pragma unroll
+    for (int i = 0; i < (S::kTokens + kRowsAtOnce - 1) / kRowsAtOnce; ++i) {
+      const int token = threadIdx.x / S::kChannels + i * kRowsAtOnce;
+      if (token >= S::kTokens || m0 + token >= M) break;
       int sum = 0;
 #pragma unroll
-      for (int v = 0; v < 8; ++v) sum += joined[v][token * kPitch + channel];
+      for (int v = 0; v < S::kSlices; ++v) sum += joined[(v * S::kTokens + token) * S::kPitch + channel];
       const float r = (float)sum * sa[m0 + token] * s;
       y[(m0 + token) * N + n] = bias ? r + shift : r;
     }
   }
 }
 
-template <int CT, int NT, int UNROLL>
+template <int CT, int NT, int TW, int UNROLL>
 int product_small(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K, float* y) {
-  const dim3 grid((unsigned)cgtb_ceil_div(N, 16 * CT), (unsigned)cgtb_ceil_div(M, 8 * NT));
-  CGTB_LAUNCH((int8_product_small_kernel<CT, NT, UNROLL>), grid, 256, 0, a, sa, b, sb, bias, M, N, K, y);
+  using S = Small<CT, NT, TW>;
+  constexpr auto kernel = int8_product_small_kernel<CT, NT, TW, UNROLL>;
+  if (S::kBytes > 48 * 1024) {
+    static const cudaError_t attribute = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (attribute != cudaSuccess) return fail("cgtb_int8_product: %s", cudaGetErrorString(attribute));
+  }
+  const dim3 grid((unsigned)cgtb_ceil_div(N, S::kChannels), (unsigned)cgtb_ceil_div(M, S::kTokens));
+  CGTB_LAUNCH(kernel, grid, 256, S::kBytes, a, sa, b, sb, bias, M, N, K, y);
   CGTB_CHECK_LAUNCH("int8_product");
   return 0;
 }
@@ -838,15 +857,22 @@ CGTB_API int cgtb_int8_product(const int8_t* a, const float* sa, const int8_t* b
     CGTB_CHECK_LAUNCH("int8_product");
     return 0;
   }
-  // Measured at N = K = 4096, M = 1, 2, 4, 16, 32: a warp per channel 5.7, 6.9, 10.4 us; 16 channels and 8 rows a block 7.9, 8.0,
-  // 8.0, 8.5, 13.3 us; tcgen05 8.9 us. N = K = 1024, M = 32, 128, 256, 512: 16 x 8 a block 2.6, 4.9, 7.4, 12.5 us, 32 x 32 3.8,
-  // 3.9, 5.0, 8.3 us, tcgen05 6.1, 6.8, 6.7, 6.8 us. 100000 rows, N = K = 64: 60 us or more against 17.
   if (M == 1) return product_rows<1>(a, sa, b, sb, bias, N, K, y);
   if (M == 2) return product_rows<2>(a, sa, b, sb, bias, N, K, y);
-  const double products = (double)M * N * K;
-  if (M <= 16 || (products <= 4e8 && M <= 1L << 18 && M * N <= 1L << 19 && N * K <= 1L << 22)) {
-    const bool larger = products > 1e8 && 2 * cgtb_ceil_div(M, 32) * cgtb_ceil_div(N, 32) >= rt().sm_count;
-    return larger ? product_small<2, 4, 2>(a, sa, b, sb, bias, M, N, K, y) : product_small<1, 1, 2>(a, sa, b, sb, bias, M, N, K, y);
+  // Measured, in us, for blocks of 16 channels x 8 rows, 16 x 16, 32 x 32, 32 x 64, and tcgen05:
+  //   8 x 4096 x 4096     7.9   8.3   9.5  14.8   8.8        128 x 4096 x 1008    -     -   7.8   6.5   8.4
+  //   32 x 4096 x 64      3.1   2.5   2.9   2.9   5.0        500 x 1001 x 1008  12.0   9.5  7.6   6.5   8.7
+  //   128 x 1024 x 1008   4.8   3.8   3.6   4.8   8.3        500 x 1001 x 2048    -     -   9.2   8.4   8.4
+  //   128 x 512 x 1008    3.2   2.8   3.6   4.8   8.3        512 x 2048 x 784     -     -  12.5  10.8   8.0
+  //   256 x 1024 x 1008   7.3   5.6   4.6   4.9   8.4        1000 x 1001 x 272    -     -   9.8   7.9   6.9
+  //   8192 x 8 x 1008     4.4   3.5   4.4   4.9    -         32 x 4096 x 4096   13.0   9.2  10.5  15.9   9.1
+  // The smaller a block, the fewer turns of its threads follow each other, and the more often the operands are read.
+  if (M <= 16 || ((double)M * N * K <= 6e8 && M <= 1L << 18 && M * N <= 1L << 19 && N * K <= 1L << 23)) {
+    const long sms = rt().sm_count, small = cgtb_ceil_div(M, 16) * cgtb_ceil_div(N, 16), middle = cgtb_ceil_div(M, 32) * cgtb_ceil_div(N, 32);
+    if (M <= 8) return product_small<1, 1, 1, 2>(a, sa, b, sb, bias, M, N, K, y);
+    if (M <= 16 || 2 * small <= 7 * sms) return product_small<1, 2, 1, 2>(a, sa, b, sb, bias, M, N, K, y);
+    if (middle <= 2 * sms) return product_small<2, 4, 1, 2>(a, sa, b, sb, bias, M, N, K, y);
+    return product_small<2, 4, 2, 2>(a, sa, b, sb, bias, M, N, K, y);
   }
   return product_tc(a, sa, b, sb, bias, M, N, K, y);
 }

@@ -212,7 +212,8 @@ int cgtb_dropout(int dtype, const void* x, long n, double p, const int64_t* stat
 
 /* Rows in 8-bit integers, x [R, C] float32: scales[r] = max_c |x[r, c]| / 127, codes[r, c] = 127 x[r, c] / max |x[r, :]| rounded
  * to the nearest whole number, ties to the even one, exactly. Rows of codes are C rounded up to a multiple of 16 long, the
- * rest zeros. A row of zeros: scale and codes 0; a row that holds an infinity or a NaN: scale NaN, codes 0. */
+ * rest zeros. A row of zeros: scale and codes 0; a row that holds an infinity or a NaN: scale NaN, codes 0. codes starts on a
+ * 16-byte boundary; x may start on any element. */
 int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, float* scales);
 /* y[m, n] = (sum_k a[m, k] * b[n, k]) * sa[m] * sb[n] + bias[n]: a product of 8-bit integers with a scale for each row of a (a
  * token) and each row of b (an output channel). a [M, K], b [N, K] int8 as cgtb_quantize_rows writes them: K a multiple of 16

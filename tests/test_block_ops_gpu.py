@@ -220,7 +220,8 @@ PRODUCTS = [(1, 1, 16), (1, 1000, 784), (1, 4096, 4096), (2, 33, 48), (4, 10, 10
             (16, 128, 128), (17, 127, 112), (31, 500, 1024), (33, 65, 96), (64, 1000, 512), (65, 17, 4112), (100, 256, 32), (127, 1, 208), (128, 128, 128),
             (129, 257, 400), (200, 300, 2064), (255, 1001, 1008), (256, 512, 64), (500, 96, 800), (1000, 10, 784), (1025, 515, 272), (3, 5000, 8192), (2500, 2100, 160),
             (300, 19000, 48), (4099, 2304, 1040), (100, 20001, 32), (2047, 4999, 16), (2, 1001, 1040),
-            (2, 10, 256), (1, 7, 8192), (3, 17, 16), (300000, 1, 32), (130, 1030, 1008), (13, 70000, 16)]
+            (2, 10, 256), (1, 7, 8192), (3, 17, 16), (300000, 1, 32), (130, 1030, 1008), (13, 70000, 16), (9, 1000, 2064), (17, 5, 1040),
+            (200000, 2, 16), (300, 1100, 96), (513, 1001, 1008), (65, 4000, 2000), (16, 8192, 4096), (32, 4099, 144)]
 
 
 def _product(a, sa, b, sb, bias):
