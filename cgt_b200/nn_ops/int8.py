@@ -20,9 +20,6 @@ class QuantizeRows(core.Op):
     available_impls = ("native_gpu",)
     results_in_variables = True
 
-    def get_diff(self, n):
-        return [False]
-
     def get_native_compile_info(self, input_types, devtype):
         return core.NativeCompileInfo(None, prebuilt="cgtb_op_quantize_rows", closure_triples=[])
 
@@ -36,13 +33,13 @@ class QuantizeRows(core.Op):
             raise ValueError("quantize_rows takes a float32 matrix, got %s" % input_types[0])
         return core.TupleType(core.TensorType("i1", 2), core.TensorType("f4", 1))
 
+    def pullback(self, inputs, output, gout):
+        raise core.NonDifferentiable("quantize_rows has no gradient")
+
 
 class Int8Product(core.Op):
     """(codes [M, K], scales [M], weight codes [N, K], weight scales [N] (, bias [N])) -> float32 [M, N]."""
     available_impls = ("native_gpu",)
-
-    def get_diff(self, n):
-        return [False] * n
 
     def get_native_compile_info(self, input_types, devtype):
         return core.NativeCompileInfo(None, prebuilt="cgtb_op_int8_product",
@@ -56,6 +53,9 @@ class Int8Product(core.Op):
         if _kinds(input_types) != want[:len(input_types)]:
             raise ValueError("int8_product takes int8 matrices and float32 vectors, got %s" % (input_types,))
         return core.TensorType("f4", 2)
+
+    def pullback(self, inputs, output, gout):
+        raise core.NonDifferentiable("int8_product has no gradient")
 
 
 def quantize_rows(x):

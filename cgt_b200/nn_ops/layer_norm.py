@@ -48,9 +48,6 @@ class LayerNormBackward(core.Op):
     def __init__(self, epsilon):
         self.epsilon = epsilon
 
-    def get_diff(self, n):
-        return [False] * n
-
     def get_native_compile_info(self, input_types, devtype):
         return core.NativeCompileInfo(None, prebuilt="cgtb_op_layer_norm_backward", closure_triples=[("epsilon", ctypes.c_double, self.epsilon)])
 
@@ -61,11 +58,15 @@ class LayerNormBackward(core.Op):
     def typ_apply(self, input_types):
         return core.TupleType(input_types[0], input_types[1], input_types[1])
 
+    def pullback(self, inputs, output, gout):
+        raise core.NonDifferentiable("layer_norm has first gradients only")
+
     def __repr__(self):
         return "LayerNormBackward{%r}" % self.epsilon
 
 
 def layer_norm(x, gain, bias, epsilon=1e-5):
     """x with every row along its last axis brought to mean 0 and variance 1, then scaled and shifted by the vectors `gain`
-    and `bias`, which have one value per column. A row of equal values gives `bias` (epsilon 0 makes it NaN)."""
+    and `bias`, which have one value per column. A row of equal values gives `bias` (epsilon 0 makes it NaN).
+    Gradients of gradients are refused."""
     return core.Result(LayerNorm(epsilon), [x, gain, bias])

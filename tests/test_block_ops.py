@@ -221,3 +221,17 @@ def test_layers_parameters():
     assert np.array_equal(q.codes.op.get_value(), codes) and np.array_equal(q.scales.op.get_value(), scales)
     assert np.array_equal(q.bias.op.get_value(), affine.bias.op.get_value()[0]) and q.codes.op.get_value().dtype == np.int8
     assert not nn.get_parameters(q(cgt.matrix("x")).sum())       # nothing to train
+
+
+def test_gradients_that_do_not_exist_are_refused_beside_others():
+    """Another way from the loss to the variable does not hide the one that has no gradient."""
+    x = cgt.shared(np.ones((3, 32), "f4"), fixed_shape_mask="all")
+    layer = nn.LayerNorm(32)
+    (dx,) = core.pullback([layer(x)], [x], [x])
+    affine = nn.Affine(32, 32)
+    (codes, scales) = nn.quantize_rows(x)
+    for loss in (cgt.square(dx).sum() + x.sum(), (nn.Int8Affine(affine)(x) + x).sum(), scales.sum() + x.sum(),
+                 nn.int8_product(codes, scales, codes, scales).sum() + x.sum()):
+        with pytest.raises(core.NonDifferentiable):
+            cgt.grad(loss, [x])
+    assert len(cgt.grad(nn.Int8Affine(affine)(x).sum() + affine(x).sum(), [affine.weight])) == 1      # x is not asked for
