@@ -36,9 +36,10 @@ struct Params {
 
 struct Tile { long m0, n0; };
 __device__ __forceinline__ Tile tile_of(const Params& p, long t) {
-  const long per = (long)kGroup * p.ntiles, g = t / per, first = g * kGroup;
-  const long rows = p.mtiles - first < kGroup ? p.mtiles - first : kGroup, r = t - g * per;
-  return Tile{(first + r % rows) * p.tile_rows, (r / rows) * p.BN};
+  // fewer than 2^31 tiles: divisions of 64 bits would take 0.1 us before the first load
+  const uint32_t per = (uint32_t)kGroup * (uint32_t)p.ntiles, g = (uint32_t)t / per, first = g * kGroup, left = (uint32_t)p.mtiles - first;
+  const uint32_t r = (uint32_t)t - g * per, rows = left < kGroup ? left : kGroup, column = left < kGroup ? r / rows : r / kGroup;
+  return Tile{(long)(first + r - column * rows) * p.tile_rows, (long)column * p.BN};
 }
 
 // D 32-bit integers, A and B signed 8-bit integers, both K-major
@@ -615,6 +616,7 @@ int product_tc(const int8_t* a, const float* sa, const int8_t* b, const float* s
   p.mtiles = (int)cgtb_ceil_div(M, p.tile_rows);
   p.ntiles = (int)cgtb_ceil_div(N, p.BN);
   p.total = (long)p.mtiles * p.ntiles;
+  if (p.total > 0x7fffffffL) return fail("cgtb_int8_product: %ld x %ld results are too many", M, N);
   p.tmem_cols = (p.split > 1 ? 1 : 2) * p.BN;
   const int a_rows = (int)std::min<long>(kRows, cgtb_ceil_div(M, 8) * 8);
   p.a_bytes = a_rows * kDepth;
