@@ -751,10 +751,7 @@ template <int CT, int NT, int TW, int UNROLL>
 int product_small(const int8_t* a, const float* sa, const int8_t* b, const float* sb, const float* bias, long M, long N, long K, float* y) {
   using S = Small<CT, NT, TW>;
   constexpr auto kernel = int8_product_small_kernel<CT, NT, TW, UNROLL>;
-  if (S::kBytes > 48 * 1024) {
-    static const cudaError_t attribute = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-    if (attribute != cudaSuccess) return fail("cgtb_int8_product: %s", cudaGetErrorString(attribute));
-  }
+  static_assert(S::kBytes <= 48 * 1024);
   const dim3 grid((unsigned)cgtb_ceil_div(N, S::kChannels), (unsigned)cgtb_ceil_div(M, S::kTokens));
   CGTB_LAUNCH(kernel, grid, 256, S::kBytes, a, sa, b, sb, bias, M, N, K, y);
   CGTB_CHECK_LAUNCH("int8_product");
