@@ -732,8 +732,10 @@ OP_BYREF(cgtb_op_dropout) {  // x, state -> y
 OP_BYREF(cgtb_op_quantize_rows) {  // x -> (codes, scales)
   cgtTuple* out = (cgtTuple*)write0;
   cgtArray *x = ARR(reads[0]), *codes = ARR(out->getitem(0)), *scales = ARR(out->getitem(1));
-  if (!all_gpu({x, codes, scales}) || x->dtype() != cgt_f4 || x->ndim() != 2 || codes->size() != x->shape()[0] * (cgtb_ceil_div(x->shape()[1], 16) * 16)) {
-    fail("QuantizeRows: takes a float32 matrix on the GPU");
+  if (!all_gpu({x, codes, scales}) || x->dtype() != cgt_f4 || x->ndim() != 2) { fail("QuantizeRows: takes a float32 matrix on the GPU"); return; }
+  const long R = x->shape()[0], padded = cgtb_ceil_div(x->shape()[1], 16) * 16;
+  if (codes->dtype() != cgt_i1 || codes->size() != R * padded || scales->dtype() != cgt_f4 || scales->size() != R) {
+    fail("QuantizeRows: the results of %ld rows are %ld codes each and a scale", R, padded);
     return;
   }
   cgtb_quantize_rows((const float*)x->data(), x->shape()[0], x->shape()[1], (int8_t*)codes->data(), (float*)scales->data());

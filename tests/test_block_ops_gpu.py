@@ -568,3 +568,19 @@ def test_one_variable_for_every_operand(rt):
         got = f()
         assert (np.abs(got[0] - want) <= by[0]).all()
         assert (np.abs(got[1] - (dx[0] + dg + db)) <= joined).all()
+
+
+@pytest.mark.parametrize("which,rows", [("scales", 3), ("scales", 9), ("codes", 3), ("dx", 3), ("dgain", 3)])
+def test_results_that_do_not_fit_their_variables_are_refused(rt, which, rows):
+    """A result may be written straight into the variable that it updates: nothing is written when the sizes differ."""
+    x, gain = _shared(np.ones((5, 16), "f4")), _shared(np.ones(16, "f4"))
+    if which in ("scales", "codes"):
+        result = nn.quantize_rows(x)[which == "scales"]
+    else:
+        result = core.pullback([nn.layer_norm(x, gain, gain * 2)], [x * 3], [x, gain])[which == "dgain"]
+    shape = {"scales": (rows,), "codes": (rows, 16), "dx": (rows, 16), "dgain": (rows,)}[which]
+    variable = cgt.shared(np.full(shape, 7, "i1" if which == "codes" else "f4"), fixed_shape_mask="all")
+    with pytest.raises(Exception):
+        cgt.function([], [], updates=[(variable, result)])()
+    assert (variable.op.get_value() == 7).all()
+    runtime.synchronize()
