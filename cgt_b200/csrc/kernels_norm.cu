@@ -736,9 +736,9 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     const long cblocks = cgtb_ceil_div(C, 256);
     P = cgtb_ceil_div(R, 64);
     if (P > 64) P = 64;
-    T* stats = (T*)scratch((size_t)(2 * R + 2 * P * C) * sizeof(T));
-    if (!stats) return 1;
-    part = stats + 2 * R;
+    part = (T*)scratch((size_t)(2 * R + 2 * P * C) * sizeof(T));    // first: the last kernel reads it 16 bytes at a time
+    if (!part) return 1;
+    T* stats = part + 2 * P * C;
     const long grid = R < rt().sm_count * 2L ? R : rt().sm_count * 2L;
     CGTB_LAUNCH(norm_backward_long_kernel<T>, (unsigned)grid, kLongThreads, 0, x, gain, gy, R, C, (T)eps, dx, stats);
     CGTB_LAUNCH(norm_columns_kernel<T>, dim3((unsigned)cblocks, (unsigned)P), 256, 0, x, gy, stats, R, C, cgtb_ceil_div(R, P), part);

@@ -584,3 +584,19 @@ def test_results_that_do_not_fit_their_variables_are_refused(rt, which, rows):
         cgt.function([], [], updates=[(variable, result)])()
     assert (variable.op.get_value() == 7).all()
     runtime.synchronize()
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("R,C,dtype", [(1, 20484, "f4"), (3, 20482, "f4"), (67, 20500, "f4"), (130, 20496, "f4"), (5, 30001, "f4"), (3, 10242, "f8"),
+                                       (65, 10244, "f8"), (7, 20481, "f8")])
+def test_gradients_of_rows_that_no_block_holds(rt, R, C, dtype, offset):
+    """Any number of them: what the kernels leave for the last one starts on 16 bytes."""
+    x, gain, bias, gy = _norm_inputs(R, C, dtype)
+    dx_, gy_ = [Dev(np.concatenate([np.zeros(offset, dtype), a.reshape(-1)])) for a in (x, gy)]
+    g = Dev(gain)
+    outs = [Dev(np.full(n + 4, 7, dtype)) for n in (R * C, C, C)]
+    call("cgtb_layer_norm_backward", code(dtype), ctypes.c_void_p(dx_.w.data + offset * x.itemsize), g.ptr,
+         ctypes.c_void_p(gy_.w.data + offset * x.itemsize), R, C, 1e-5, *[o.ptr for o in outs])
+    for (o, want, bound) in zip(outs, ref.norm_gradients(x, gain, gy, 1e-5), ref.norm_bounds(x, gain, bias, gy, 1e-5)[1:]):
+        flat = o.get()
+        assert (np.abs(flat[:want.size].reshape(want.shape) - want) <= bound).all() and (flat[want.size:] == 7).all()
