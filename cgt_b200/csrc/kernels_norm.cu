@@ -101,7 +101,7 @@ __device__ __forceinline__ void team_sums(T (&s)[K], T* part, int turn) {
 }
 
 __device__ __forceinline__ float inverse_root(float v) { return 1.0f / sqrtf(v); }
-__device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ double inverse_root(double v) { return rsqrt(v); }
 
 // ================================================================================================
 // Layer norm: y = (x - m) / sqrt(v + eps) * gain + bias with the row's mean m and variance v (of the centred values, so
