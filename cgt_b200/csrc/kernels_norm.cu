@@ -100,6 +100,11 @@ __device__ __forceinline__ void team_sums(T (&s)[K], T* part, int turn) {
   }
 }
 
+// v / C. A division of float64 is a long chain of dependent steps, so there it is a product with 1 / C, one rounding more (gradients of
+// 100000 x 65: 43.6 -> 36.6 us); in float32 it is not the slower one (8192 x 4096: 69 us, with a product 72 us). The mean, which
+// everything else is centred around, is divided in both.
+__device__ __forceinline__ float share(float v, int C, float) { return v / (float)C; }
+__device__ __forceinline__ double share(double v, int, double inverse) { return v * inverse; }
 __device__ __forceinline__ float inverse_root(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double inverse_root(double v) { return rsqrt(v); }
 
@@ -122,6 +127,7 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
   b.load(bias, C, t, T(0));
   // all teams of a block make the same number of steps: they share barriers
   const long step = (long)gridDim.x * kTeams;
+  const T inverse = T(1) / (T)C;      // float64
   long r = (long)blockIdx.x * kTeams + team;
   if (r < R) next.load(x + r * C, C, t, T(0));
   for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
       q[0] += inside[e / VEC] ? row.v[e] * row.v[e] : T(0);
     }
     team_sums<TEAM>(q, part, 1);
-    const T rstd = inverse_root(q[0] / (T)C + eps);
+    const T rstd = inverse_root(share(q[0], C, inverse) + eps);
     if (r < R) {
 #pragma unroll
       for (int e = 0; e < E; ++e) row.v[e] = row.v[e] * rstd * g.v[e] + b.v[e];
@@ -259,6 +265,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   };
+  const T inverse = T(1) / (T)C;      // float64
   long r = (long)blockIdx.x * kTeams + team;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) fetch(i, (VEC == 1 ? (long)blockIdx.x * kTeams : r) + i * step);
@@ -315,7 +322,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       s[1] += g.v[e] * w.v[e];
     }
     team_sums<TEAM>(s, sums, 0);
-    const T mean = s[0] / (T)C, s1 = s[1] / (T)C;
+    const T mean = s[0] / (T)C, s1 = share(s[1], C, inverse);
     T q[2] = {T(0), T(0)};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -324,7 +331,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       q[1] += g.v[e] * w.v[e] * a.v[e];      // g is 0 beyond C
     }
     team_sums<TEAM>(q, sums, 1);
-    const T rstd = inverse_root(q[0] / (T)C + eps), s2 = q[1] / (T)C * rstd;
+    const T rstd = inverse_root(share(q[0], C, inverse) + eps), s2 = share(q[1], C, inverse) * rstd;
     if (r < R) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
