@@ -182,8 +182,8 @@ __device__ __forceinline__ Part part_of_row(int C) {
 }
 
 // The sums of all blocks of a cluster from theirs, in the blocks' order; every thread gets them. Every block is told the others' by
-// stores that count their bytes at its barrier: nothing is released, so no store of results is waited for (with barriers of the
-// whole cluster 1677 x 19999 takes 182 us instead of 110). Consecutive calls alternate `turn`, and the threads of a block meet
+// stores that count their bytes at its barrier: nothing is released, so no store of results is waited for (barriers of the
+// whole cluster: 1677 x 19999 182 us, then 110, now 96). Consecutive calls alternate `turn`, and the threads of a block meet
 // between two calls: a block that is told the sums of a row's turn again has read those before, since it told its own since then.
 constexpr int kMaxCluster = 8;
 template <typename T, bool SHARED, int K>
@@ -230,7 +230,9 @@ __device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       T t = space.slots[turn][0][k];
-      for (int q = 1; q < mine.blocks; ++q) t += space.slots[turn][q][k];
+#pragma unroll
+      for (int q = 1; q < kMaxCluster; ++q)      // all loads at once: a loop over the blocks costs 15 us at 1677 x 19999
+        if (q < mine.blocks) t += space.slots[turn][q][k];
       s[k] = t;
     }
   }
@@ -758,8 +760,8 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   else failed = norm_backward_teams<T, 64 / sizeof(T), 512>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
   if (failed > 0) return 1;
   // Rows that no team holds, by clusters: their blocks hold 32 or 16 KB of a row, of which two fit an SM. The larger ones are faster
-  // where the row fills them as well (2000 x 16384: 83 and 101 us), the smaller ones where it does not (3000 x 9001: 117 and 113
-  // us, 1677 x 20000: 143 and 103 us).
+  // where the row fills them as well (2000 x 16384: 84 and 101 us), the smaller ones where it does not (1677 x 20000: 143 and 103
+  // us, before the sums' loads were made at once, which takes another tenth off).
   constexpr long kLarge = 512 * (64 / sizeof(T)), kSmall = kLarge / 2;
   auto clusters = [&](auto threads, int blocks) {
     constexpr int TEAM = decltype(threads)::value, E = 64 / sizeof(T);
