@@ -109,52 +109,6 @@ __device__ __forceinline__ double share(double v, int, double inverse) { return 
 __device__ __forceinline__ float inverse_root(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double inverse_root(double v) { return rsqrt(v); }
 
-// ================================================================================================
-// Layer norm: y = (x - m) / sqrt(v + eps) * gain + bias with the row's mean m and variance v (of the centred values, so
-// that a large common offset costs no digits). Bound by the bytes of x and y: every row is read once, and the next row's loads
-// are under way while this row's sums are formed.
-// ================================================================================================
-template <typename T, int VEC, int N, int TEAM>
-__global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
-                                                                          long R, int C, T eps, T* __restrict__ y) {
-  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
-  __shared__ T part[2 * (kBlock / 32) * 1];
-  const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
-  Row<T, VEC, N, TEAM> g, b, row, next;
-  bool inside[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) inside[i] = (i * TEAM + t) * VEC < C;
-  g.load(gain, C, t, T(0));
-  b.load(bias, C, t, T(0));
-  // all teams of a block make the same number of steps: they share barriers
-  const long step = (long)gridDim.x * kTeams;
-  const T inverse = T(1) / (T)C;      // float64
-  long r = (long)blockIdx.x * kTeams + team;
-  if (r < R) next.load(x + r * C, C, t, T(0));
-  for (long first = (long)blockIdx.x * kTeams; first < R; first += step, r += step) {
-    row = next;
-    if (r + step < R) next.load(x + (r + step) * C, C, t, T(0));
-    T s[1] = {T(0)};
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += row.v[e];
-    team_sums<TEAM>(s, part, 0);
-    const T mean = s[0] / (T)C;
-    T q[1] = {T(0)};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      row.v[e] -= mean;
-      q[0] += inside[e / VEC] ? row.v[e] * row.v[e] : T(0);
-    }
-    team_sums<TEAM>(q, part, 1);
-    const T rstd = inverse_root(share(q[0], C, inverse) + eps);
-    if (r < R) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) row.v[e] = row.v[e] * rstd * g.v[e] + b.v[e];
-      row.store(y + r * C, C, t);
-    }
-  }
-}
-
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -182,8 +136,8 @@ __device__ __forceinline__ Part part_of_row(int C) {
 }
 
 // The sums of all blocks of a cluster from theirs, in the blocks' order; every thread gets them. Every block is told the others' by
-// stores that count their bytes at its barrier: nothing is released, so no store of results is waited for (barriers of the
-// whole cluster: 1677 x 19999 182 us, then 110, now 96). Consecutive calls alternate `turn`, and the threads of a block meet
+// stores that count their bytes at its barrier: nothing is released, so no store of results is waited for (with barriers of
+// the whole cluster 1677 x 19999 took 182 us, with these stores 110). Consecutive calls alternate `turn`, and the threads of a block meet
 // between two calls: a block that is told the sums of a row's turn again has read those before, since it told its own since then.
 constexpr int kMaxCluster = 8;
 template <typename T, bool SHARED, int K>
@@ -236,6 +190,60 @@ __device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, 
       s[k] = t;
     }
   }
+}
+
+// ================================================================================================
+// Layer norm: y = (x - m) / sqrt(v + eps) * gain + bias with the row's mean m and variance v (of the centred values, so
+// that a large common offset costs no digits). Bound by the bytes of x and y: every row is read once, and the next row's loads
+// are under way while this row's sums are formed.
+// ================================================================================================
+template <typename T, int VEC, int N, int TEAM, bool SHARED>
+__global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
+                                                                          long R, int C, T eps, T* __restrict__ y, int* err) {
+  constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
+  __shared__ T part[2 * (kBlock / 32) * 1];
+  __shared__ ClusterSpace<T, SHARED, 1> space;
+  const Part mine = part_of_row<SHARED>(C);
+  uint32_t parity = 0;
+  const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+  Row<T, VEC, N, TEAM> g, b, row, next;
+  bool inside[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) inside[i] = (i * TEAM + t) * VEC < mine.count;
+  g.load(gain + mine.first, mine.count, t, T(0));
+  b.load(bias + mine.first, mine.count, t, T(0));
+  cluster_begin(space);
+  // all teams of a block make the same number of steps: they share barriers
+  const long group = blockIdx.x / mine.blocks, step = (long)(gridDim.x / mine.blocks) * kTeams;
+  const T inverse = T(1) / (T)C;      // float64
+  long r = group * kTeams + team;
+  if (r < R) next.load(x + r * C + mine.first, mine.count, t, T(0));
+  for (long first = group * kTeams; first < R; first += step, r += step) {
+    row = next;
+    if (r + step < R) next.load(x + (r + step) * C + mine.first, mine.count, t, T(0));
+    T s[1] = {T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0] += row.v[e];
+    team_sums<TEAM>(s, part, 0);
+    cluster_sums(s, space, mine, 0, parity, err);
+    const T mean = s[0] / (T)C;
+    T q[1] = {T(0)};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      row.v[e] -= mean;
+      q[0] += inside[e / VEC] ? row.v[e] * row.v[e] : T(0);
+    }
+    team_sums<TEAM>(q, part, 1);
+    cluster_sums(q, space, mine, 1, parity, err);
+    parity ^= 1u;
+    const T rstd = inverse_root(share(q[0], C, inverse) + eps);
+    if (r < R) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) row.v[e] = row.v[e] * rstd * g.v[e] + b.v[e];
+      row.store(y + r * C + mine.first, mine.count, t);
+    }
+  }
+  if (SHARED) cluster_sync();      // no block leaves while it may be told something
 }
 
 // One element group of a thread from global to shared memory, asynchronously
@@ -499,50 +507,9 @@ void norm_fold(const T* part, long C, long P, T* dgain, T* dbias) {
   else CGTB_LAUNCH((norm_fold_kernel<T, 1>), (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
 }
 
-// ---- longer rows, up to 20480 float32 or 10240 float64: a block of 1024 threads holds one, 20 or 10 elements a thread, and has
-// no registers for more than that. gain and bias are read again for every row (from the L2 cache). One row of 80 KB per SM is
-// enough under way at a time: float32 1677 x 20000 63 us, 69 us by clusters as the gradients have them, 92 us by the kernel below.
 constexpr int kLongThreads = 1024;
-template <typename T> constexpr int wide_elements() { return 80 / sizeof(T); }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kLongThreads) norm_forward_wide_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
-                                                                         long R, int C, T eps, T* __restrict__ y) {
-  constexpr int E = wide_elements<T>(), N = E / VEC;
-  typedef Pack<T, VEC> P;
-  __shared__ T part[2 * 32];
-  const int t = threadIdx.x;
-  for (long r = blockIdx.x; r < R; r += gridDim.x) {
-    Row<T, VEC, N, kLongThreads> row;
-    row.load(x + r * C, C, t, T(0));
-    T s[1] = {T(0)};
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += row.v[e];
-    team_sums<kLongThreads>(s, part, 0);
-    const T mean = s[0] / (T)C;
-    T q[1] = {T(0)};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      row.v[e] -= mean;
-      if ((e / VEC * kLongThreads + t) * VEC < C) q[0] += row.v[e] * row.v[e];
-    }
-    team_sums<kLongThreads>(q, part, 1);
-    const T rstd = inverse_root(q[0] / (T)C + eps);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * kLongThreads + t) * VEC;
-      if (c < C) {
-        const P g = *reinterpret_cast<const P*>(gain + c), b = *reinterpret_cast<const P*>(bias + c);
-        P p;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p.v[j] = row.v[i * VEC + j] * rstd * g.v[j] + b.v[j];
-        *reinterpret_cast<P*>(y + r * C + c) = p;
-      }
-    }
-  }
-}
-
-// ---- rows that no team holds: a block per row that reads it several times (the L2 cache has it) ----
+// ---- rows that no cluster holds: a block per row that reads it several times (the L2 cache has it) ----
 template <typename T>
 __device__ __forceinline__ void long_row_statistics(const T* x, long C, T eps, T* part, T& mean, T& rstd) {
   T s[1] = {T(0)};
@@ -647,7 +614,7 @@ long resident_blocks() {
 // Launches KERNEL, whose clusters of `blocks` blocks walk the rows, with as many of them as the GPU holds at a time; returns their
 // number, 0 when it failed.
 template <auto KERNEL, int THREADS, size_t BYTES, typename F>
-long launch_clusters(int blocks, long R, F arguments) {
+long launch_clusters(const char* who, int blocks, long R, F arguments) {
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)blocks;
@@ -670,7 +637,7 @@ long launch_clusters(int blocks, long R, F arguments) {
   config.gridDim = dim3((unsigned)(P * blocks));
   const cudaError_t e = arguments(config, P);
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-  if (e != cudaSuccess) { fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e)); return 0; }
+  if (e != cudaSuccess) { fail("%s launch failed: %s", who, cudaGetErrorString(e)); return 0; }
   return P;
 }
 
@@ -681,18 +648,28 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   const bool held = with_team<E, 1024>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
     auto launch = [&](auto width, auto elements) {
-      constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, decltype(elements)::value / decltype(width)::value, TEAM>;
+      constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, decltype(elements)::value / decltype(width)::value, TEAM, false>;
       const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
-      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y);
+      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y, (int*)nullptr);
     };
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>(), std::integral_constant<int, E>());
     else if (TEAM > 1 && C <= TEAM * (E * 3 / 4)) launch(std::integral_constant<int, 1>(), std::integral_constant<int, E * 3 / 4>());     // fewer places without an element
     else launch(std::integral_constant<int, 1>(), std::integral_constant<int, E>());
   });
-  if (!held && C <= kLongThreads * wide_elements<T>()) {
-    const unsigned grid = (unsigned)std::min<long>(R, rt().sm_count);
-    if (wide) CGTB_LAUNCH((norm_forward_wide_kernel<T, 16 / sizeof(T)>), grid, kLongThreads, 0, x, gain, bias, R, (int)C, (T)eps, y);
-    else CGTB_LAUNCH((norm_forward_wide_kernel<T, 1>), grid, kLongThreads, 0, x, gain, bias, R, (int)C, (T)eps, y);
+  // Rows that no team holds, by clusters whose blocks hold 16 KB of a row: 1677 x 19999 66 us, 3000 x 9001 63 us (a block of 1024
+  // threads for a row: 76 and 78 us; blocks of 512 threads and 16 KB 81 and 79 us).
+  constexpr int kTeam = 256, kElements = 64 / sizeof(T);
+  if (!held && C <= 1L * kTeam * kElements * kMaxCluster) {
+    int* const err = tc_error_flag();
+    if (!err) return 1;
+    auto launch = [&](auto width) {
+      constexpr int VEC = decltype(width)::value;
+      constexpr auto kernel = norm_forward_kernel<T, VEC, kElements / VEC, kTeam, true>;
+      return launch_clusters<kernel, kTeam, 0>("layer_norm_forward", (int)cgtb_ceil_div(C, kTeam * kElements), R, [&](const cudaLaunchConfig_t& config, long) {
+        return cudaLaunchKernelEx(&config, kernel, x, gain, bias, R, (int)C, (T)eps, y, err);
+      });
+    };
+    if (!(wide ? launch(std::integral_constant<int, 16 / sizeof(T)>()) : launch(std::integral_constant<int, 1>()))) return 1;
   } else if (!held) {
     const unsigned grid = (unsigned)std::min<long>(R, rt().sm_count * 2L);
     CGTB_LAUNCH(norm_forward_long_kernel<T>, grid, kLongThreads, 0, x, gain, bias, R, C, (T)eps, y);
@@ -760,8 +737,8 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   else failed = norm_backward_teams<T, 64 / sizeof(T), 512>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
   if (failed > 0) return 1;
   // Rows that no team holds, by clusters: their blocks hold 32 or 16 KB of a row, of which two fit an SM. The larger ones are faster
-  // where the row fills them as well (2000 x 16384: 84 and 101 us), the smaller ones where it does not (1677 x 20000: 143 and 103
-  // us, before the sums' loads were made at once, which takes another tenth off).
+  // where the row fills them as well (2000 x 16384: 84 and 101 us), the smaller ones where it does not (1677 x 20000, before the
+  // sums of a cluster were loaded at once: 143 and 103 us).
   constexpr long kLarge = 512 * (64 / sizeof(T)), kSmall = kLarge / 2;
   auto clusters = [&](auto threads, int blocks) {
     constexpr int TEAM = decltype(threads)::value, E = 64 / sizeof(T);
@@ -769,7 +746,7 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     constexpr auto kernel = norm_backward_kernel<T, 1, E, TEAM, false, true>;
     int* const err = tc_error_flag();
     if (!err) return 0L;
-    return launch_clusters<kernel, TEAM, bytes>(blocks, R, [&](const cudaLaunchConfig_t& config, long n) {
+    return launch_clusters<kernel, TEAM, bytes>("layer_norm_backward", blocks, R, [&](const cudaLaunchConfig_t& config, long n) {
       part = (T*)scratch((size_t)n * 2 * C * sizeof(T));
       return part ? cudaLaunchKernelEx(&config, kernel, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, err) : cudaErrorMemoryAllocation;
     });

@@ -600,3 +600,21 @@ def test_gradients_of_rows_that_no_block_holds(rt, R, C, dtype, offset):
     for (o, want, bound) in zip(outs, ref.norm_gradients(x, gain, gy, 1e-5), ref.norm_bounds(x, gain, bias, gy, 1e-5)[1:]):
         flat = o.get()
         assert (np.abs(flat[:want.size].reshape(want.shape) - want) <= bound).all() and (flat[want.size:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("R,C", [(1, 4097), (300, 8193), (2, 8196), (41, 12289), (200, 16384), (3, 16385), (2, 20001), (90, 24580), (1, 32768), (3, 32769)])
+def test_layer_norm_of_rows_that_blocks_share(rt, R, C, dtype):
+    """Rows of two to eight blocks, at the sizes where their number changes, more rows than clusters and fewer."""
+    test_layer_norm(rt, R, C, dtype)
+
+
+def test_long_rows_are_the_same_in_every_call(rt):
+    """Blocks that share a row add its sums in one order: no bit differs between calls, eager or replayed."""
+    R, C = 40, 20001
+    x, gain, bias, gy = [_shared(a) for a in _norm_inputs(R, C, "f4")]
+    y = nn.layer_norm(x, gain, bias)
+    f = cgt.function([], [y] + core.pullback([y], [gy], [x, gain, bias]))
+    first = [a.copy() for a in f()]
+    for _ in range(6):
+        assert all(np.array_equal(a, b) for (a, b) in zip(f(), first))
