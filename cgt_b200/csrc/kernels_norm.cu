@@ -657,7 +657,8 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
     else launch(std::integral_constant<int, 1>(), std::integral_constant<int, E>());
   });
   // Rows that no team holds, by clusters whose blocks hold 16 KB of a row: 1677 x 19999 66 us, 3000 x 9001 63 us (a block of 1024
-  // threads for a row: 76 and 78 us; blocks of 512 threads and 16 KB 81 and 79 us).
+  // threads for a row: 76 and 78 us; blocks of 512 threads and 16 KB 81 and 79 us). Where one block holds the row it is faster
+  // (4096 x 8192 49 us, by clusters 52; gradients 69 and 84 us).
   constexpr int kTeam = 256, kElements = 64 / sizeof(T);
   if (!held && C <= 1L * kTeam * kElements * kMaxCluster) {
     int* const err = tc_error_flag();
