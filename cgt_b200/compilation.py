@@ -2573,10 +2573,11 @@ def _copy(node):
 
 def copy_shared_targets(updatetargs, node2shape):
     """An update target is computed in its variable's memory: one instruction per variable. A value that several variables
-    get, and one that is a view of something else (a reshape, some rows), is copied into the variable."""
+    get, one that no instruction computes (another variable, an argument), and one that is a view of something else (a
+    reshape, some rows) is copied into the variable."""
     (out, seen) = ([], set())
     for t in updatetargs:
-        if t in seen or (not t.is_input() and t.op.return_type == "byval"):
+        if t in seen or t.is_input() or t.op.return_type == "byval":
             copy = _copy(t)
             copy.props.update(t.props)
             node2shape[copy] = node2shape[t]

@@ -200,3 +200,20 @@ def test_one_value_for_several_variables_and_views_as_values():
     _same_as_oracle([x], [c - new], [(a, new), (b, new), (c, new)])
     _same_as_oracle([y], [a * 2.0], [(a, cgt.tanh(y).reshape([6, 6]))])
     _same_as_oracle([], [a * 2.0, b * 3.0], [(a, cgt.concatenate([b, b], axis=0)[3:9]), (b, b - a)])
+
+
+@pytest.mark.parametrize("read", [False, True])
+def test_variables_and_arguments_as_values(read):
+    """A variable that gets another variable or an argument as it is, whether or not the function reads it otherwise, two
+    that change places, and one that gets itself."""
+    rs = np.random.RandomState(0)
+    (a, b, c, d) = [_var(rs, 6, 6) for _ in range(4)]
+    (x, outputs) = (cgt.matrix("x", fixed_shape=(6, 6)), [a + b * c] if read else [])
+    _same_as_oracle([], outputs, [(a, b)])
+    _same_as_oracle([x], outputs, [(a, x)])
+    _same_as_oracle([x], outputs, [(a, b), (b, c), (c, x)])
+    _same_as_oracle([x], outputs, [(a, b), (b, a), (c, x), (d, x)])
+    _same_as_oracle([], outputs, [(a, b), (b, a + c), (c, a), (d, d)])
+    (s, t) = [cgt.shared(np.array(k, "f4"), device=core.Device("cpu", 0)) for k in (2, 7)]
+    _same_as_oracle([], outputs, [(s, t), (t, s * 2.0)])
+    _same_as_oracle([], outputs, [(s, t)])

@@ -70,3 +70,19 @@ def test_against_the_oracle(rt, build):
         for (i, (got, want)) in enumerate(pairs):
             # sums of at most K terms in another order, carried on through the steps; 8 for what cancels
             assert np.linalg.norm(got - want) <= 8 * K * steps * np.finfo("f4").eps * max(np.linalg.norm(want), 1e-3), (step, i)
+
+
+@pytest.mark.parametrize("read", [False, True])
+def test_variables_and_arguments_as_values(rt, read):
+    """Variables that get another variable or an argument as it is, two that change places, eager and replayed."""
+    rs = np.random.RandomState(0)
+    (a, b, c, d) = [_var(rs, 50, 30) for _ in range(4)]
+    x = cgt.matrix("x", fixed_shape=(50, 30))
+    values = [v.op.get_value() for v in (a, b, c, d)]
+    f = cgt.function([x], [a * 2.0] if read else [x * 1.0], updates=[(a, b), (b, a), (c, x), (d, c)])
+    for step in range(6):
+        arg = rs.randn(50, 30).astype("f4")
+        got = f(arg)[0]
+        assert np.array_equal(got, values[0] * 2 if read else arg)
+        values = [values[1], values[0], arg, values[2]]
+        assert all(np.array_equal(v.op.get_value(), w) for (v, w) in zip((a, b, c, d), values)), step
