@@ -7,7 +7,11 @@ import numpy as np
 from .. import core
 
 PAD = 16               # rows of codes are a multiple of this long, so that every row starts on a 16-byte boundary
-MAX_CODES = 131072     # of one row: the sums are 32-bit integers
+MAX_CODES = 131072     # a row, with its padding, has fewer: the sums are 32-bit integers
+
+
+def _padded(columns):
+    return -(-columns // PAD) * PAD
 
 
 def _kinds(types):
@@ -67,7 +71,7 @@ def quantize_rows(x):
 
 def int8_product(codes, scales, weight_codes, weight_scales, bias=None):
     """codes.dot(weight_codes.T), exact, times the scale of the row and that of the output channel, plus `bias`: float32
-    [rows, channels]. Both matrices of codes as ``quantize_rows`` returns them."""
+    [rows, channels]. Both matrices of codes as ``quantize_rows`` returns them; rows of up to 131056 codes."""
     return core.Result(Int8Product(), [codes, scales, weight_codes, weight_scales] + ([] if bias is None else [bias]))
 
 
@@ -80,8 +84,8 @@ class Int8Affine(object):
         weight = affine.weight.op.get_value()
         if weight.dtype != np.float32:
             raise ValueError("Int8Affine takes a float32 layer, got %s" % weight.dtype)
-        if len(weight) >= MAX_CODES:
-            raise ValueError("Int8Affine takes a layer of fewer than %d inputs, got %d" % (MAX_CODES, len(weight)))
+        if _padded(len(weight)) >= MAX_CODES:
+            raise ValueError("Int8Affine takes a layer of up to %d inputs, got %d" % (MAX_CODES - PAD, len(weight)))
         codes, scales = _quantize(weight.T)
         shared = core.cgt.shared
         self.codes = shared(codes, fixed_shape_mask="all")
@@ -99,6 +103,6 @@ def _quantize(x):
     finite = np.isfinite(largest)
     with np.errstate(all="ignore"):
         ratio = 127 * x.astype("f8") / np.where(largest > 0, largest, 1).astype("f8")
-    codes = np.zeros((x.shape[0], -(-x.shape[1] // PAD) * PAD), "i1")
+    codes = np.zeros((x.shape[0], _padded(x.shape[1])), "i1")
     codes[:, :x.shape[1]] = np.rint(np.where(finite, ratio, 0)).astype("i1")
     return codes, np.where(finite, largest / np.float32(127), np.float32(np.nan))[:, 0].astype("f4")

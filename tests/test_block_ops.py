@@ -235,3 +235,11 @@ def test_gradients_that_do_not_exist_are_refused_beside_others():
         with pytest.raises(core.NonDifferentiable):
             cgt.grad(loss, [x])
     assert len(cgt.grad(nn.Int8Affine(affine)(x).sum() + affine(x).sum(), [affine.weight])) == 1      # x is not asked for
+
+
+def test_the_longest_layer_in_8_bits():
+    """131056 inputs are the longest row of codes that a product takes; one more is padded to 131072, which none does."""
+    assert nn.Int8Affine(nn.Affine(131056, 1)).codes.op.get_value().shape == (1, 131056)
+    for inputs in (131057, 131071):
+        with pytest.raises(ValueError, match="up to 131056 inputs"):
+            nn.Int8Affine(nn.Affine(inputs, 1))
