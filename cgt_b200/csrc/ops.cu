@@ -752,8 +752,8 @@ OP_BYREF(cgtb_op_int8_product) {  // codes, scales, weight codes, weight scales 
   }
   const long M = a->shape()[0], N = b->shape()[0];
   if (sa->size() != M || sb->size() != N || (bias && bias->size() != N) || y->size() != M * N || sa->dtype() != cgt_f4 || sb->dtype() != cgt_f4 ||
-      (bias && bias->dtype() != cgt_f4)) {
-    fail("Int8Product: needs a float32 scale for each of the %ld rows and each of the %ld output channels", M, N);
+      y->dtype() != cgt_f4 || (bias && bias->dtype() != cgt_f4)) {
+    fail("Int8Product: needs a float32 scale for each of the %ld rows and each of the %ld output channels, and a float32 result", M, N);
     return;
   }
   cgtb_int8_product((const int8_t*)a->data(), (const float*)sa->data(), (const int8_t*)b->data(), (const float*)sb->data(),

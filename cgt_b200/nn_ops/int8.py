@@ -19,6 +19,13 @@ def _kinds(types):
     return [(t.dtype, t.ndim) for t in types]
 
 
+def _float32(ndim):
+    """The type of a float32 array, whatever the configured precision: the kernels write nothing else."""
+    t = core.TensorType("f4", ndim)
+    t.dtype = "f4"
+    return t
+
+
 class QuantizeRows(core.Op):
     """(x float32 [R, C]) -> codes int8 [R, C up to a multiple of 16] and scales float32 [R]."""
     available_impls = ("native_gpu",)
@@ -35,7 +42,7 @@ class QuantizeRows(core.Op):
     def typ_apply(self, input_types):
         if _kinds(input_types) != [("f4", 2)]:
             raise ValueError("quantize_rows takes a float32 matrix, got %s" % input_types[0])
-        return core.TupleType(core.TensorType("i1", 2), core.TensorType("f4", 1))
+        return core.TupleType(core.TensorType("i1", 2), _float32(1))
 
     def pullback(self, inputs, output, gout):
         raise core.NonDifferentiable("quantize_rows has no gradient")
@@ -56,7 +63,7 @@ class Int8Product(core.Op):
         want = [("i1", 2), ("f4", 1)] * 2 + [("f4", 1)]
         if _kinds(input_types) != want[:len(input_types)]:
             raise ValueError("int8_product takes int8 matrices and float32 vectors, got %s" % (input_types,))
-        return core.TensorType("f4", 2)
+        return _float32(2)
 
     def pullback(self, inputs, output, gout):
         raise core.NonDifferentiable("int8_product has no gradient")

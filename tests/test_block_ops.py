@@ -243,3 +243,15 @@ def test_the_longest_layer_in_8_bits():
     for inputs in (131057, 131071):
         with pytest.raises(ValueError, match="up to 131056 inputs"):
             nn.Int8Affine(nn.Affine(inputs, 1))
+
+
+def test_8_bit_results_are_float32_in_every_precision():
+    """Variables of one precision in a graph that is built or compiled under the other: the kernels know float32 only."""
+    x, w = cgt.shared(np.ones((3, 20), "f4"), fixed_shape_mask="all"), cgt.shared(np.ones((4, 32), "i1"), fixed_shape_mask="all")
+    s = cgt.shared(np.ones(4, "f4"), fixed_shape_mask="all")
+    with cgt.scoped_update_config(precision="double"):
+        codes, scales = nn.quantize_rows(x)
+        y = nn.int8_product(codes, scales, w, s)
+        assert scales.dtype == "f4" and y.dtype == "f4"
+        eg = compilation.execution_graph([], [y], [], [])[0]
+    assert all(i.dtype[0] != "f" or i.dtype == "f4" for i in eg.instrs if isinstance(i, compilation.Alloc))

@@ -618,3 +618,17 @@ def test_long_rows_are_the_same_in_every_call(rt):
     first = [a.copy() for a in f()]
     for _ in range(6):
         assert all(np.array_equal(a, b) for (a, b) in zip(f(), first))
+
+
+def test_8_bit_layers_under_the_other_precision(rt):
+    """Float32 variables in a function that is built and compiled in double precision: the same float32 results."""
+    rs = np.random.RandomState(0)
+    x, wv = rs.randn(6, 40).astype("f4"), rs.randn(9, 40).astype("f4")
+    rows, w, sw = _shared(x), _shared(ref.quantize(wv)[0]), _shared(ref.quantize(wv)[1])
+    with cgt.scoped_update_config(precision="double"):
+        codes, scales = nn.quantize_rows(rows)
+        f = cgt.function([], [nn.int8_product(codes, scales, w, sw)])
+    want, bound = ref.product(*ref.quantize(x), *ref.quantize(wv), None)
+    for _ in range(4):
+        got = f()[0]
+        assert got.dtype == np.float32 and (np.abs(got - want) <= bound).all()
