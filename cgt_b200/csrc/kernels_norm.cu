@@ -56,6 +56,29 @@ struct Row {
 constexpr int kTeamThreads = 256;   // of a block, unless a team is larger
 template <int TEAM> constexpr int team_block() { return TEAM > kTeamThreads ? TEAM : kTeamThreads; }
 
+// Waits for other blocks or for copies are bounded: after `cycles` a thread raises the error flag, the block's `note` of it and kGaveUp
+// among its own flags. A thread that has given up, or waits and finds the note, waits no more; thread 0 then asks for no copies, and
+// the threads that tell the other blocks something tell them nothing. The block runs through its rows, whose results are
+// invalid: it waits in vain once, however many rows there are.
+struct Waits {
+  int* err;
+  uint32_t cycles;
+  uint32_t flags;      // of every thread at first; kSilent: nothing is asked for or told, so that every wait is in vain (a self-test)
+};
+constexpr uint32_t kGaveUp = 1u << 31, kSilent = 1u << 30;
+__device__ __forceinline__ bool wait_until(uint32_t bar, uint32_t parity, const Waits& waits, volatile int* note, uint32_t& flags) {
+  if (flags & kGaveUp) return false;
+  if (tc::mbar_try(bar, parity)) return true;
+  const uint32_t t0 = (uint32_t)clock();
+  while (!*note && (uint32_t)clock() - t0 < waits.cycles)
+    if (tc::mbar_try(bar, parity)) return true;
+  flags |= kGaveUp;
+  *note = 1;
+  *(volatile int*)waits.err = 9;
+  __threadfence_system();
+  return false;
+}
+
 // Sums of one or two values over a team, in a fixed order; every thread gets them. `part`: the block's space for teams of several
 // warps, 2 * K * (warps of the block) values; consecutive calls alternate `turn`, so that one barrier separates a call's reads
 // from the next but one's writes. Two values cost little more than one: after the first step half of the lanes go on with
@@ -144,11 +167,13 @@ template <typename T, bool SHARED, int K>
 struct ClusterSpace {
   T slots[2][SHARED ? kMaxCluster : 1][K];
   uint64_t told[2];
+  int note;
 };
 template <typename T, bool SHARED, int K>
 __device__ __forceinline__ void cluster_begin(ClusterSpace<T, SHARED, K>& space) {
   if constexpr (SHARED) {
     if (threadIdx.x == 0) {
+      space.note = 0;
       tc::mbar_init(tc::smem_u32(&space.told[0]), 1);
       tc::mbar_init(tc::smem_u32(&space.told[1]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -158,11 +183,15 @@ __device__ __forceinline__ void cluster_begin(ClusterSpace<T, SHARED, K>& space)
   }
 }
 template <typename T, bool SHARED, int K>
-__device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, K>& space, const Part& mine, int turn, uint32_t parity, int* err) {
+__device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, K>& space, const Part& mine, int turn, uint32_t parity, const Waits& waits,
+                                             uint32_t& flags) {
   if constexpr (SHARED) {
     const uint32_t bar = tc::smem_u32(&space.told[turn]);
-    if (threadIdx.x == 0) tc::mbar_arrive_expect_tx(bar, mine.blocks * K * (uint32_t)sizeof(T));
-    if (threadIdx.x < mine.blocks) {
+    // A thread that has not waited in vain knows that the last use of the barrier is over, and that the others have read the sums
+    // that they were told before
+    const bool tell = flags < kSilent;
+    if (threadIdx.x == 0 && tell) tc::mbar_arrive_expect_tx(bar, mine.blocks * K * (uint32_t)sizeof(T));
+    if (threadIdx.x < mine.blocks && tell) {
       uint32_t at, there;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(&space.slots[turn][mine.rank][0])), "r"((uint32_t)threadIdx.x));
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"((uint32_t)threadIdx.x));
@@ -173,13 +202,10 @@ __device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, 
         else asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f64 [%0], %1, [%2];" ::"r"(at + k * 8), "d"(s[k]), "r"(there) : "memory");
       }
     }
-    uint32_t seen = tc::mbar_wait(bar, parity);      // bounded; the sums are invalid when it expires
-    if (seen)      // and what the other blocks stored is visible
+    if (wait_until(bar, parity, waits, &space.note, flags)) {     // this makes what the other blocks stored visible
+      uint32_t seen;
       asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
                    : "=r"(seen) : "r"(bar), "r"(parity) : "memory");
-    if (!seen) {
-      *(volatile int*)err = 9;
-      __threadfence_system();
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -192,6 +218,18 @@ __device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, 
   }
 }
 
+// The end of a cluster's kernel: no block leaves while it may be told something. What it has not waited for is on its way at most
+// when all blocks are here.
+template <typename T, bool SHARED, int K>
+__device__ __forceinline__ void cluster_end(ClusterSpace<T, SHARED, K>& space) {
+  if constexpr (SHARED) {
+    __syncwarp();
+    cluster_sync();
+    const uint32_t t0 = (uint32_t)clock();
+    while (*(volatile int*)&space.note && (uint32_t)clock() - t0 < 2000000u) __nanosleep(1000);
+  }
+}
+
 // ================================================================================================
 // Layer norm: y = (x - m) / sqrt(v + eps) * gain + bias with the row's mean m and variance v (of the centred values, so
 // that a large common offset costs no digits). Bound by the bytes of x and y: every row is read once, and the next row's loads
@@ -199,12 +237,12 @@ __device__ __forceinline__ void cluster_sums(T (&s)[K], ClusterSpace<T, SHARED, 
 // ================================================================================================
 template <typename T, int VEC, int N, int TEAM, bool SHARED>
 __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ bias,
-                                                                          long R, int C, T eps, T* __restrict__ y, int* err) {
+                                                                          long R, int C, T eps, T* __restrict__ y, const Waits waits) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
   __shared__ T part[2 * (kBlock / 32) * 1];
   __shared__ ClusterSpace<T, SHARED, 1> space;
   const Part mine = part_of_row<SHARED>(C);
-  uint32_t parity = 0;
+  uint32_t flags = waits.flags;      // and the parity of the sums' exchanges
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
   Row<T, VEC, N, TEAM> g, b, row, next;
   bool inside[N];
@@ -225,7 +263,7 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
 #pragma unroll
     for (int e = 0; e < E; ++e) s[0] += row.v[e];
     team_sums<TEAM>(s, part, 0);
-    cluster_sums(s, space, mine, 0, parity, err);
+    cluster_sums(s, space, mine, 0, flags & 1u, waits, flags);
     const T mean = s[0] / (T)C;
     T q[1] = {T(0)};
 #pragma unroll
@@ -234,8 +272,8 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
       q[0] += inside[e / VEC] ? row.v[e] * row.v[e] : T(0);
     }
     team_sums<TEAM>(q, part, 1);
-    cluster_sums(q, space, mine, 1, parity, err);
-    parity ^= 1u;
+    cluster_sums(q, space, mine, 1, flags & 1u, waits, flags);
+    flags ^= 1u;
     const T rstd = inverse_root(share(q[0], C, inverse) + eps);
     if (r < R) {
 #pragma unroll
@@ -243,7 +281,7 @@ __global__ void __launch_bounds__(team_block<TEAM>()) norm_forward_kernel(const 
       row.store(y + r * C + mine.first, mine.count, t);
     }
   }
-  if (SHARED) cluster_sync();      // no block leaves while it may be told something
+  cluster_end(space);
 }
 
 // One element group of a thread from global to shared memory, asynchronously
@@ -293,14 +331,14 @@ __device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t b
 template <typename T, int VEC, int N, int TEAM, bool ONE, bool SHARED>
 __global__ void __launch_bounds__(team_block<TEAM>(), (TEAM == 1024 || VEC * N * sizeof(T) == 32 && sizeof(T) == 4 ? 1024 : 512) / team_block<TEAM>())
 norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const T* __restrict__ gy, long R, int C, T eps, T* __restrict__ dx,
-                     T* __restrict__ part, T* __restrict__ dgain, T* __restrict__ dbias, int* err) {
+                     T* __restrict__ part, T* __restrict__ dgain, T* __restrict__ dbias, const Waits waits) {
   constexpr int kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM, E = VEC * N;
   typedef Pack<T, VEC> P;
   extern __shared__ __align__(16) unsigned char ahead_raw[];
   __shared__ __align__(16) T sums[2 * (kBlock / 32) * 2];
   __shared__ ClusterSpace<T, SHARED, 2> space;
-  uint32_t parity = 0;
   __shared__ __align__(8) uint64_t full[kAhead + 1];
+  uint32_t flags = waits.flags;      // bits 0 to kAhead: phases of the stages' barriers; bit 8: parity of the sums' exchanges
   constexpr size_t kArray = norm_backward_array<T, VEC, N, TEAM>();
   P* ahead = reinterpret_cast<P*>(ahead_raw) + threadIdx.x;     // [kAhead + 1][x, gy][N][thread]
   const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
@@ -315,6 +353,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
         for (int j = 0; j < VEC; ++j) ahead[(k * N + i) * kBlock].v[j] = T(0);
   }
   if (VEC == 1 && threadIdx.x == 0) {
+    space.note = 0;
     for (int i = 0; i <= kAhead; ++i) tc::mbar_init(tc::smem_u32(&full[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -326,7 +365,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
         const long rows = R - r < kTeams ? R - r : kTeams;
         const long count = !SHARED ? rows * C : mine.count;
         const Span<T> sx(x, R * C, r * C + mine.first, count), sg(gy, R * C, r * C + mine.first, count);
-        if (sx.inside && sg.inside) {
+        if (sx.inside && sg.inside && flags < kSilent) {      // the copy before it into this place has landed
           const uint32_t bar = tc::smem_u32(&full[stage]);
           tc::mbar_arrive_expect_tx(bar, sx.bytes + sg.bytes);
           copy_bulk(ahead_raw + (stage * 2) * kArray, sx.from, sx.bytes, bar);
@@ -357,7 +396,6 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
 #pragma unroll
   for (int e = 0; e < E; ++e) dg.v[e] = db.v[e] = T(0);
   int stage = 0;
-  uint32_t phases = 0;       // of the stages' barriers
   for (long first = group * kTeams; first < R; first += step, r += step) {
     // VEC 1: the stage that is filled now was read in the step before; teams of several warps met at a barrier since
     if (VEC == 1 && TEAM <= 32) __syncthreads();
@@ -368,11 +406,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       const long count = !SHARED ? rows * C : mine.count;
       const Span<T> sx(x, R * C, first * C + mine.first, count), sg(gy, R * C, first * C + mine.first, count);
       if (sx.inside && sg.inside) {
-        if (!tc::mbar_wait(tc::smem_u32(&full[stage]), (phases >> stage) & 1u)) {     // bounded; the sums are invalid then
-          *(volatile int*)err = 9;
-          __threadfence_system();
-        }
-        phases ^= 1u << stage;
+        if (wait_until(tc::smem_u32(&full[stage]), (flags >> stage) & 1u, waits, &space.note, flags)) flags ^= 1u << stage;
         const T* from_x = reinterpret_cast<const T*>(ahead_raw + (stage * 2) * kArray + sx.shift) + team * C + t;
         const T* from_g = reinterpret_cast<const T*>(ahead_raw + (stage * 2 + 1) * kArray + sg.shift) + team * C + t;
 #pragma unroll
@@ -406,7 +440,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       s[1] += g.v[e] * w.v[e];
     }
     team_sums<TEAM>(s, sums, 0);
-    cluster_sums(s, space, mine, 0, parity, err);
+    cluster_sums(s, space, mine, 0, flags >> 8 & 1u, waits, flags);
     const T mean = s[0] / (T)C, s1 = share(s[1], C, inverse);
     T q[2] = {T(0), T(0)};
 #pragma unroll
@@ -416,8 +450,8 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       q[1] += g.v[e] * w.v[e] * a.v[e];      // g is 0 beyond C
     }
     team_sums<TEAM>(q, sums, 1);
-    cluster_sums(q, space, mine, 1, parity, err);
-    parity ^= 1u;
+    cluster_sums(q, space, mine, 1, flags >> 8 & 1u, waits, flags);
+    flags ^= 1u << 8;
     const T rstd = inverse_root(share(q[0], C, inverse) + eps), s2 = share(q[1], C, inverse) * rstd;
     if (r < R) {
 #pragma unroll
@@ -433,6 +467,11 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
   // ONE, for few rows: the whole grid is one cluster, whose blocks leave their sums in their shared memory and then add all
   // blocks' sums of a share of the columns, in order; no second kernel.
   T* joined = reinterpret_cast<T*>(ahead_raw);      // 2 E of the block's threads, or 2 C: less than the rows took
+  if (VEC == 1 && threadIdx.x == 0 && flags >= kSilent)      // copies that were not waited for land before their place is written or left
+    for (int i = 0; i <= kAhead; ++i) {
+      const uint32_t t0 = (uint32_t)clock();
+      while (!tc::mbar_try(tc::smem_u32(&full[i]), (flags >> i) & 1u) && (uint32_t)clock() - t0 < 20000000u) {}
+    }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (kTeams > 1 || ONE) __syncthreads();
   T* out = ONE ? joined + (kTeams > 1 ? 2 * E * kBlock : 0) : part + group * 2 * C;
@@ -455,7 +494,7 @@ norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ gain, const 
       if (c < C) out[(long)which * C + c] = v;
     }
   }
-  if (SHARED) cluster_sync();      // no block leaves while it may be told something
+  cluster_end(space);
   if constexpr (ONE) {
     cluster_sync();
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(out);
@@ -641,6 +680,12 @@ long launch_clusters(const char* who, int blocks, long R, F arguments) {
   return P;
 }
 
+std::atomic<uint32_t> g_selftest_cycles{0};
+Waits bounded_waits() {
+  const uint32_t cycles = g_selftest_cycles.load();
+  return Waits{tc_error_flag(), cycles ? cycles : (uint32_t)tc::kWaitCycles, cycles ? kSilent : 0u};
+}
+
 template <typename T>
 int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, double eps, T* y) {
   constexpr int E = 32 / sizeof(T);     // 8 float32 or 4 float64 a thread
@@ -650,7 +695,7 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
     auto launch = [&](auto width, auto elements) {
       constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, decltype(elements)::value / decltype(width)::value, TEAM, false>;
       const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
-      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y, (int*)nullptr);
+      CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y, Waits());
     };
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>(), std::integral_constant<int, E>());
     else if (TEAM > 1 && C <= TEAM * (E * 3 / 4)) launch(std::integral_constant<int, 1>(), std::integral_constant<int, E * 3 / 4>());     // fewer places without an element
@@ -661,13 +706,13 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   // (4096 x 8192 49 us, by clusters 52; gradients 69 and 84 us).
   constexpr int kTeam = 256, kElements = 64 / sizeof(T);
   if (!held && C <= 1L * kTeam * kElements * kMaxCluster) {
-    int* const err = tc_error_flag();
-    if (!err) return 1;
+    const Waits waits = bounded_waits();
+    if (!waits.err) return 1;
     auto launch = [&](auto width) {
       constexpr int VEC = decltype(width)::value;
       constexpr auto kernel = norm_forward_kernel<T, VEC, kElements / VEC, kTeam, true>;
       return launch_clusters<kernel, kTeam, 0>("layer_norm_forward", (int)cgtb_ceil_div(C, kTeam * kElements), R, [&](const cudaLaunchConfig_t& config, long) {
-        return cudaLaunchKernelEx(&config, kernel, x, gain, bias, R, (int)C, (T)eps, y, err);
+        return cudaLaunchKernelEx(&config, kernel, x, gain, bias, R, (int)C, (T)eps, y, waits);
       });
     };
     if (!(wide ? launch(std::integral_constant<int, 16 / sizeof(T)>()) : launch(std::integral_constant<int, 1>()))) return 1;
@@ -683,8 +728,9 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
 // is that large
 template <typename T, int E, int kMaxTeam>
 int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, bool wide, T* dx, T* dgain, T* dbias, T*& part, long& P) {
-  int failed = 0, *const err = tc_error_flag();
-  if (!err) return 1;
+  int failed = 0;
+  const Waits waits = bounded_waits();
+  if (!waits.err) return 1;
   const bool held = with_team<E, kMaxTeam>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
     auto launch = [&](auto width) {
@@ -705,7 +751,7 @@ int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, 
         config.stream = rt().stream;
         config.attrs = &attr;
         config.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias, err);
+        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias, waits);
         if (e != cudaSuccess) failed = fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e));
         g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
         return;
@@ -715,7 +761,7 @@ int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, 
       P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
       part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
       if (!part) failed = 1;
-      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, err);
+      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, waits);
     };
     if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
     else launch(std::integral_constant<int, 1>());
@@ -745,11 +791,11 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
     constexpr int TEAM = decltype(threads)::value, E = 64 / sizeof(T);
     constexpr size_t bytes = norm_backward_bytes<T, 1, E, TEAM>();
     constexpr auto kernel = norm_backward_kernel<T, 1, E, TEAM, false, true>;
-    int* const err = tc_error_flag();
-    if (!err) return 0L;
+    const Waits waits = bounded_waits();
+    if (!waits.err) return 0L;
     return launch_clusters<kernel, TEAM, bytes>("layer_norm_backward", blocks, R, [&](const cudaLaunchConfig_t& config, long n) {
       part = (T*)scratch((size_t)n * 2 * C * sizeof(T));
-      return part ? cudaLaunchKernelEx(&config, kernel, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, err) : cudaErrorMemoryAllocation;
+      return part ? cudaLaunchKernelEx(&config, kernel, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, waits) : cudaErrorMemoryAllocation;
     });
   };
   if (failed < 0 && C <= kSmall * kMaxCluster) {
@@ -987,6 +1033,12 @@ CGTB_API int cgtb_layer_norm_backward(int dtype, const void* x, const void* gain
   if (dtype == cgtb_f4)
     return norm_backward((const float*)x, (const float*)gain, (const float*)gy, R, C, epsilon, (float*)dx, (float*)dgain, (float*)dbias);
   return norm_backward((const double*)x, (const double*)gain, (const double*)gy, R, C, epsilon, (double*)dx, (double*)dgain, (double*)dbias);
+}
+
+CGTB_API int cgtb_layer_norm_selftest_waits(long cycles) {
+  if (cycles < 0 || cycles > (long)tc::kWaitCycles) return fail("cgtb_layer_norm_selftest_waits: 0 to %ld cycles", (long)tc::kWaitCycles);
+  g_selftest_cycles.store((uint32_t)cycles);
+  return 0;
 }
 
 CGTB_API int cgtb_dropout(int dtype, const void* x, long n, double p, const int64_t* state, unsigned site, void* y) {

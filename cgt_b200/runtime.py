@@ -91,6 +91,7 @@ def _declare(lib):
         "cgtb_lrn_backward": (ci, [ci, vp, vp, vp, vp, cl, ci, ci, ci, ci, cd, cd, vp]),
         "cgtb_layer_norm_forward": (ci, [ci, vp, cl, cl, vp, vp, cd, vp]),
         "cgtb_layer_norm_backward": (ci, [ci, vp, vp, vp, cl, cl, cd, vp, vp, vp]),
+        "cgtb_layer_norm_selftest_waits": (ci, [cl]),
         "cgtb_dropout": (ci, [ci, vp, cl, cd, vp, ctypes.c_uint, vp]),
         "cgtb_quantize_rows": (ci, [vp, cl, cl, vp, vp]), "cgtb_int8_product": (ci, [vp, vp, vp, vp, vp, cl, cl, cl, vp]),
         "cgtb_conv_dgrad": (ci, [vp, cl, ci, ci, ci, vp] + [ci] * 7 + [vp]),

@@ -202,6 +202,11 @@ int cgtb_lrn_backward(int dtype, const void* x, const void* top, const void* sca
 int cgtb_layer_norm_forward(int dtype, const void* x, long R, long C, const void* gain, const void* bias, double epsilon, void* y);
 int cgtb_layer_norm_backward(int dtype, const void* x, const void* gain, const void* gy, long R, long C, double epsilon, void* dx,
                              void* dgain, void* dbias);
+/* The blocks of these kernels wait for copies into their shared memory and, where several share a row, for each other's sums. A
+ * wait lasts about a second at most; then the call's results are invalid, the kernel ends without waiting any more, and the next
+ * synchronisation reports it. cgtb_layer_norm_selftest_waits, for tests: with cycles > 0 every such wait is in vain and gives up after
+ * that many SM clock cycles, with 0 the kernels are as they were. */
+int cgtb_layer_norm_selftest_waits(long cycles);
 
 /* Dropout of n values, float32 or float64: y[i] = x[i] / (1 - p), or 0 where the element is dropped, whatever x[i] is. No mask
  * is stored: element i is dropped where word i % 4 of the Philox4x32-10 block with key (seed, seed >> 32) and counter

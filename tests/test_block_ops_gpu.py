@@ -1,6 +1,7 @@
 """Layer norm, dropout, 8-bit rows and 8-bit products on the GPU against tests/block_ops.py, at the sizes where the kernels
 change their form, and in compiled functions."""
 import ctypes
+import time
 
 import numpy as np
 import pytest
@@ -632,3 +633,45 @@ def test_8_bit_layers_under_the_other_precision(rt):
     for _ in range(4):
         got = f()[0]
         assert got.dtype == np.float32 and (np.abs(got - want) <= bound).all()
+
+
+IN_VAIN = [("forward", 2500, 9001, "f4"), ("forward", 2500, 5000, "f8"), ("backward", 400000, 17, "f4"), ("backward", 40000, 301, "f8"), ("backward", 10000, 2047, "f4"),
+           ("backward", 3000, 3001, "f8"), ("backward", 2500, 9001, "f4"), ("backward", 2500, 9001, "f8"), ("backward", 7, 1001, "f4")]
+
+
+@pytest.mark.parametrize("which,R,C,dtype", IN_VAIN)
+def test_a_block_waits_in_vain_once(rt, which, R, C, dtype):
+    """No copy arrives and no block is told anything: the kernels end by themselves after one limit, not one for each of a
+    block's eight or more rows, the failure is reported, and the library stays usable."""
+    L = runtime.lib()
+    rs = np.random.RandomState(0)
+    x, gy = rs.randn(R, C).astype(dtype), rs.randn(R, C).astype(dtype)
+    gain, bias = rs.randn(C).astype(dtype), rs.randn(C).astype(dtype)
+    dx, dgy, dg, db = Dev(x), Dev(gy), Dev(gain), Dev(bias)
+    out, sums = Dev(np.full((R, C), 7, dtype)), [Dev(np.zeros(C, dtype)) for _ in range(2)]
+
+    def run():
+        if which == "forward":
+            assert L.cgtb_layer_norm_forward(code(dtype), dx.ptr, R, C, dg.ptr, db.ptr, 1e-5, out.ptr) == 0
+        else:
+            assert L.cgtb_layer_norm_backward(code(dtype), dx.ptr, dg.ptr, dgy.ptr, R, C, 1e-5, out.ptr, *[s.ptr for s in sums]) == 0
+        return L.cgtb_synchronize()
+    cycles = 100_000_000                 # 0.05 s or a little more; a copy that is still awaited at the end costs three times 0.01 s
+    runtime.check(L.cgtb_layer_norm_selftest_waits(cycles), "selftest")
+    try:
+        start = time.monotonic()
+        failed = run()
+        seconds = time.monotonic() - start
+    finally:
+        runtime.check(L.cgtb_layer_norm_selftest_waits(0), "selftest")
+    assert failed and "code 9" in runtime.last_error()
+    assert seconds < 0.25, seconds       # eight rows with a wait each: 0.4 s
+    assert run() == 0
+    got = out.get()
+    some = slice(0, R, max(1, R // 50))
+    if which == "forward":
+        want, bound = ref.norm(x[some], gain, bias, 1e-5)[0], ref.norm_bounds(x[some], gain, bias, None, 1e-5)
+    else:
+        want, bound = ref.norm_gradients(x[some], gain, gy[some], 1e-5)[0], ref.norm_bounds(x[some], gain, bias, gy[some], 1e-5)[1]
+    assert (np.abs(got[some] - want) <= bound).all()
+    assert L.cgtb_layer_norm_selftest_waits(-1) != 0 and L.cgtb_layer_norm_selftest_waits(1 << 40) != 0
