@@ -497,8 +497,9 @@ int sgemm_tc_check() {
   if (g_err_host && *g_err_host) {
     int code = *g_err_host;
     *g_err_host = 0;
-    return fail("a bounded device-side wait expired (code %d: 3-7 a barrier of the tensor-core GEMM / convolution kernels, 8 a rank "
-                "of the peer-memory all-reduce did not arrive, 9 a copy of layer norm's gradients); the result of that call is invalid", code);
+    return fail("a bounded device-side wait expired (code %d: 3-7 a barrier of the tensor-core GEMM, convolution and 8-bit product "
+                "kernels, 8 a rank of the peer-memory all-reduce did not arrive, 9 layer norm's copy of a row or another block's sums "
+                "of it); the result of that call is invalid", code);
   }
   return 0;
 }

@@ -675,3 +675,23 @@ def test_a_block_waits_in_vain_once(rt, which, R, C, dtype):
         want, bound = ref.norm_gradients(x[some], gain, gy[some], 1e-5)[0], ref.norm_bounds(x[some], gain, bias, gy[some], 1e-5)[1]
     assert (np.abs(got[some] - want) <= bound).all()
     assert L.cgtb_layer_norm_selftest_waits(-1) != 0 and L.cgtb_layer_norm_selftest_waits(1 << 40) != 0
+
+
+@pytest.mark.parametrize("R,C", [(6, 1000), (6, 9001)])
+def test_what_is_said_of_a_wait_in_vain(rt, R, C):
+    """The forward pass waits for other blocks only, the gradients of short rows for copies only: the text names both."""
+    L = runtime.lib()
+    x, gain, bias, gy = [Dev(a) for a in _norm_inputs(R, C + 1, "f4")]
+    out, sums = Dev(np.zeros((R, C + 1), "f4")), [Dev(np.zeros(C + 1, "f4")) for _ in range(2)]
+    runtime.check(L.cgtb_layer_norm_selftest_waits(100_000), "selftest")
+    try:
+        if C > 8192:
+            assert L.cgtb_layer_norm_forward(code("f4"), x.ptr, R, C + 1, gain.ptr, bias.ptr, 1e-5, out.ptr) == 0
+        else:
+            assert L.cgtb_layer_norm_backward(code("f4"), x.ptr, gain.ptr, gy.ptr, R, C + 1, 1e-5, out.ptr, *[d.ptr for d in sums]) == 0
+        failed = L.cgtb_synchronize()
+    finally:
+        runtime.check(L.cgtb_layer_norm_selftest_waits(0), "selftest")
+    text = runtime.last_error()
+    assert failed and "code 9" in text and "8-bit product" in text and "copy of a row or another block's sums" in text
+    runtime.synchronize()
