@@ -541,9 +541,13 @@ __global__ void __launch_bounds__(32 * kFoldGroups) norm_fold_kernel(const T* __
 }
 template <typename T>
 void norm_fold(const T* part, long C, long P, T* dgain, T* dbias) {
-  constexpr int VEC = 16 / sizeof(T);
-  if (2 * C % VEC == 0) CGTB_LAUNCH((norm_fold_kernel<T, VEC>), (unsigned)cgtb_ceil_div(2 * C, 32 * VEC), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
-  else CGTB_LAUNCH((norm_fold_kernel<T, 1>), (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
+  constexpr int VEC = 16 / sizeof(T);      // float64: 2, of which 2 C is a multiple
+  if constexpr (VEC > 2)
+    if (2 * C % VEC) {
+      CGTB_LAUNCH((norm_fold_kernel<T, 1>), (unsigned)cgtb_ceil_div(2 * C, 32), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
+      return;
+    }
+  CGTB_LAUNCH((norm_fold_kernel<T, VEC>), (unsigned)cgtb_ceil_div(2 * C, 32 * VEC), 32 * kFoldGroups, 0, part, C, (int)P, dgain, dbias);
 }
 
 constexpr int kLongThreads = 1024;
@@ -618,24 +622,16 @@ template <typename T> bool starts_on_16(long C, std::initializer_list<const void
   return true;
 }
 
-// calls f(team) with the smallest team for rows of C elements, E of them a thread; false when none is large enough
-template <int E, int kMaxTeam, typename F>
+// calls f(team) with the smallest team for rows of C elements, E of them a thread; false when none is large enough. Only teams from
+// kMinTeam to kMaxTeam are made; where kMinTeam is above 1, the caller has rows that no smaller team holds.
+template <int E, int kMinTeam, int kMaxTeam, typename F>
 bool with_team(long C, F f) {
-  if (C <= 1L * E) f(std::integral_constant<int, 1>());
-  else if (C <= 2L * E) f(std::integral_constant<int, 2>());
-  else if (C <= 4L * E) f(std::integral_constant<int, 4>());
-  else if (C <= 8L * E) f(std::integral_constant<int, 8>());
-  else if (C <= 16L * E) f(std::integral_constant<int, 16>());
-  else if (C <= 32L * E) f(std::integral_constant<int, 32>());
-  else if (C <= 64L * E) f(std::integral_constant<int, 64>());
-  else if (C <= 128L * E) f(std::integral_constant<int, 128>());
-  else {
-    if constexpr (kMaxTeam >= 256) { if (C <= 256L * E) { f(std::integral_constant<int, 256>()); return true; } }
-    if constexpr (kMaxTeam >= 512) { if (C <= 512L * E) { f(std::integral_constant<int, 512>()); return true; } }
-    if constexpr (kMaxTeam >= 1024) { if (C <= 1024L * E) { f(std::integral_constant<int, 1024>()); return true; } }
-    return false;
+  if (C <= (long)kMinTeam * E) {
+    f(std::integral_constant<int, kMinTeam>());
+    return true;
   }
-  return true;
+  if constexpr (kMinTeam < kMaxTeam) return with_team<E, 2 * kMinTeam, kMaxTeam>(C, f);
+  else return false;
 }
 
 // as many blocks as the SMs hold at a time: the grid of a kernel whose blocks walk the rows
@@ -690,16 +686,17 @@ template <typename T>
 int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, double eps, T* y) {
   constexpr int E = 32 / sizeof(T);     // 8 float32 or 4 float64 a thread
   const bool wide = starts_on_16<T>(C, {x, gain, bias, y});
-  const bool held = with_team<E, 1024>(C, [&](auto team) {
+  const bool held = with_team<E, 1, 1024>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>();
     auto launch = [&](auto width, auto elements) {
       constexpr auto kernel = norm_forward_kernel<T, decltype(width)::value, decltype(elements)::value / decltype(width)::value, TEAM, false>;
       const long blocks = std::min<long>(cgtb_ceil_div(R, kBlock / TEAM), resident_blocks<kernel, kBlock, 0>());
       CGTB_LAUNCH(kernel, (unsigned)blocks, kBlock, 0, x, gain, bias, R, (int)C, (T)eps, y, Waits());
     };
-    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>(), std::integral_constant<int, E>());
-    else if (TEAM > 1 && C <= TEAM * (E * 3 / 4)) launch(std::integral_constant<int, 1>(), std::integral_constant<int, E * 3 / 4>());     // fewer places without an element
-    else launch(std::integral_constant<int, 1>(), std::integral_constant<int, E>());
+    if (wide) return launch(std::integral_constant<int, 16 / sizeof(T)>(), std::integral_constant<int, E>());
+    if constexpr (TEAM > 1)      // fewer places without an element
+      if (C <= TEAM * (E * 3 / 4)) return launch(std::integral_constant<int, 1>(), std::integral_constant<int, E * 3 / 4>());
+    launch(std::integral_constant<int, 1>(), std::integral_constant<int, E>());
   });
   // Rows that no team holds, by clusters whose blocks hold 16 KB of a row: 1677 x 19999 66 us, 3000 x 9001 63 us (a block of 1024
   // threads for a row: 76 and 78 us; blocks of 512 threads and 16 KB 81 and 79 us). Where one block holds the row it is faster
@@ -724,47 +721,42 @@ int norm_forward(const T* x, long R, long C, const T* gain, const T* bias, doubl
   return 0;
 }
 
-// The gradients by teams of E elements a thread; dgain and dbias are complete, or in `part` for P blocks. 1: failed, -1: no team
-// is that large
-template <typename T, int E, int kMaxTeam>
-int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, bool wide, T* dx, T* dgain, T* dbias, T*& part, long& P) {
+// The gradients by teams of E elements a thread, VEC at a time; dgain and dbias are complete, or in `part` for P blocks. 1: failed,
+// -1: no team is that large
+template <typename T, int VEC, int E, int kMinTeam, int kMaxTeam>
+int norm_backward_teams(const T* x, const T* gain, const T* gy, long R, long C, double eps, T* dx, T* dgain, T* dbias, T*& part, long& P) {
   int failed = 0;
   const Waits waits = bounded_waits();
   if (!waits.err) return 1;
-  const bool held = with_team<E, kMaxTeam>(C, [&](auto team) {
+  const bool held = with_team<E, kMinTeam, kMaxTeam>(C, [&](auto team) {
     constexpr int TEAM = decltype(team)::value, kBlock = team_block<TEAM>(), kTeams = kBlock / TEAM;
-    auto launch = [&](auto width) {
-      constexpr int VEC = decltype(width)::value;
-      constexpr size_t bytes = norm_backward_bytes<T, VEC, E / VEC, TEAM>();
-      constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM, false, false>, one = norm_backward_kernel<T, VEC, E / VEC, TEAM, true, false>;
-      const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
-      if (steps <= 8) {       // (512 x 256, 32 steps: 7.0 us by eight blocks, 5.1 us by more and another kernel)
-        (void)resident_blocks<one, kBlock, bytes>();      // allows the shared memory
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = steps > 4 ? 8 : steps > 2 ? 4 : steps > 1 ? 2 : 1;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cudaLaunchConfig_t config = {};
-        config.gridDim = dim3(attr.val.clusterDim.x);
-        config.blockDim = dim3(kBlock);
-        config.dynamicSmemBytes = bytes;
-        config.stream = rt().stream;
-        config.attrs = &attr;
-        config.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias, waits);
-        if (e != cudaSuccess) failed = fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e));
-        g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-        return;
-      }
-      // at least four rows for a team, so that what the blocks leave for the last kernel stays small against the rows; but no SM
-      // without a block where there are rows for it
-      P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
-      part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
-      if (!part) failed = 1;
-      else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, waits);
-    };
-    if (wide) launch(std::integral_constant<int, 16 / sizeof(T)>());
-    else launch(std::integral_constant<int, 1>());
+    constexpr size_t bytes = norm_backward_bytes<T, VEC, E / VEC, TEAM>();
+    constexpr auto kernel = norm_backward_kernel<T, VEC, E / VEC, TEAM, false, false>, one = norm_backward_kernel<T, VEC, E / VEC, TEAM, true, false>;
+    const long steps = cgtb_ceil_div(R, kTeams), sms = rt().sm_count;
+    if (steps <= 8) {       // (512 x 256, 32 steps: 7.0 us by eight blocks, 5.1 us by more and another kernel)
+      (void)resident_blocks<one, kBlock, bytes>();      // allows the shared memory
+      cudaLaunchAttribute attr = {};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = steps > 4 ? 8 : steps > 2 ? 4 : steps > 1 ? 2 : 1;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(attr.val.clusterDim.x);
+      config.blockDim = dim3(kBlock);
+      config.dynamicSmemBytes = bytes;
+      config.stream = rt().stream;
+      config.attrs = &attr;
+      config.numAttrs = 1;
+      const cudaError_t e = cudaLaunchKernelEx(&config, one, x, gain, gy, R, (int)C, (T)eps, dx, (T*)nullptr, dgain, dbias, waits);
+      if (e != cudaSuccess) failed = fail("layer_norm_backward launch failed: %s", cudaGetErrorString(e));
+      g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+      return;
+    }
+    // at least four rows for a team, so that what the blocks leave for the last kernel stays small against the rows; but no SM
+    // without a block where there are rows for it
+    P = std::min(std::min(steps, resident_blocks<kernel, kBlock, bytes>()), std::max(cgtb_ceil_div(steps, 4), sms));
+    part = (T*)scratch((size_t)P * 2 * C * sizeof(T));     // starts on a 256-byte boundary
+    if (!part) failed = 1;
+    else CGTB_LAUNCH(kernel, (unsigned)P, kBlock, bytes, x, gain, gy, R, (int)C, (T)eps, dx, part, (T*)nullptr, (T*)nullptr, waits);
   });
   return held ? failed : -1;
 }
@@ -778,10 +770,28 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   // that start on 16-byte boundaries are read 16 bytes at a time (100000 x 64: 20 against 31 us, 4000 x 5000: 53 against 66 us),
   // but in between, where two or four rows are under way on an SM, by the bulk copies all the same (8192 x 4096: 69 against 86 us).
   const bool starts = starts_on_16<T>(C, {x, gain, gy, dx});
-  const bool wide = starts && (sizeof(T) == 8 ? C <= 1024 : C <= 1024 || C > 4096);
+  auto teams = [&](auto width, auto elements, auto least, auto most) {
+    return norm_backward_teams<T, decltype(width)::value, decltype(elements)::value, decltype(least)::value, decltype(most)::value>(
+        x, gain, gy, R, C, eps, dx, dgain, dbias, part, P);
+  };
+  constexpr std::integral_constant<int, 16 / sizeof(T)> k16Bytes;
+  constexpr std::integral_constant<int, 1> kOne;
+  constexpr std::integral_constant<int, 32 / sizeof(T)> kFew;
+  constexpr std::integral_constant<int, 64 / sizeof(T)> kMany;
+  constexpr std::integral_constant<int, 512> kLargest;
+  constexpr std::integral_constant<int, 16 / kFew> kUpTo16;         // the team that holds 16 columns, and the least one for more of them
+  constexpr std::integral_constant<int, 32 / kMany> kFrom17;
   int failed;
-  if (C <= 16 || (sizeof(T) == 8 && wide)) failed = norm_backward_teams<T, 32 / sizeof(T), 256>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
-  else failed = norm_backward_teams<T, 64 / sizeof(T), 512>(x, gain, gy, R, C, eps, wide, dx, dgain, dbias, part, P);
+  if constexpr (sizeof(T) == 8) {
+    if (starts && C <= 1024) failed = teams(k16Bytes, kFew, kOne, std::integral_constant<int, 1024 / kFew>());
+    else if (C <= 16) failed = teams(kOne, kFew, kOne, kUpTo16);
+    else failed = teams(kOne, kMany, kFrom17, kLargest);
+  } else {
+    if (C <= 16) failed = starts ? teams(k16Bytes, kFew, kOne, kUpTo16) : teams(kOne, kFew, kOne, kUpTo16);
+    else if (starts && C <= 1024) failed = teams(k16Bytes, kMany, kFrom17, std::integral_constant<int, 1024 / kMany>());
+    else if (starts && C > 4096) failed = teams(k16Bytes, kMany, kLargest, kLargest);
+    else failed = teams(kOne, kMany, kFrom17, kLargest);
+  }
   if (failed > 0) return 1;
   // Rows that no team holds, by clusters: their blocks hold 32 or 16 KB of a row, of which two fit an SM. The larger ones are faster
   // where the row fills them as well (2000 x 16384: 84 and 101 us), the smaller ones where it does not (1677 x 20000, before the
@@ -1074,7 +1084,7 @@ CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, f
     if (wide) launch(std::true_type(), elements, team);
     else launch(std::false_type(), elements, team);
   };
-  bool held = with_team<16, 1024>(Cp, [&](auto team) { either(std::integral_constant<int, 16>(), team); });
+  bool held = with_team<16, 1, 1024>(Cp, [&](auto team) { either(std::integral_constant<int, 16>(), team); });
   if (!held && Cp <= 1024 * 20) {
     either(std::integral_constant<int, 20>(), std::integral_constant<int, 1024>());
     held = true;

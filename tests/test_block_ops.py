@@ -1,10 +1,14 @@
 """Layer norm, dropout, 8-bit rows and 8-bit products without a GPU: the generator's published answers, refusals when a
 graph is built, and which memory a step's results go to."""
+import re
+import shutil
+import subprocess
+
 import numpy as np
 import pytest
 
 import cgt_b200 as cgt
-from cgt_b200 import compilation, core, nn
+from cgt_b200 import build, compilation, core, nn
 from cgt_b200.nn_ops import dropout as dropout_ops
 from cgt_b200.nn_ops import int8 as int8_ops
 from cgt_b200.nn_ops import layer_norm as norm_ops
@@ -255,3 +259,50 @@ def test_8_bit_results_are_float32_in_every_precision():
         assert scales.dtype == "f4" and y.dtype == "f4"
         eg = compilation.execution_graph([], [y], [], [])[0]
     assert all(i.dtype[0] != "f" or i.dtype == "f4" for i in eg.instrs if isinstance(i, compilation.Alloc))
+
+
+def _norm_kernels(C, kind, aligned):
+    """The layer norm kernels that may be launched for rows of C elements of `kind`, which start on 16-byte boundaries or not."""
+    size = {"float": 4, "double": 8}[kind]
+    starts = aligned and C * size % 16 == 0
+    names = set()
+
+    def team(elements, most):
+        return next((t for t in (1 << k for k in range(11)) if t <= most and C <= t * elements), None)
+    E = 32 // size
+    t = team(E, 1024)
+    if t:
+        E = E if starts or t == 1 or C > t * (E * 3 // 4) else E * 3 // 4
+        vec = 16 // size if starts else 1
+        names.add("norm_forward_kernel<%s, %d, %d, %d, false>" % (kind, vec, E // vec, t))
+    elif C <= 256 * (64 // size) * 8:
+        vec = 16 // size if starts else 1
+        names.add("norm_forward_kernel<%s, %d, %d, 256, true>" % (kind, vec, 64 // size // vec))
+    else:
+        names.add("norm_forward_long_kernel<%s>" % kind)
+    wide = starts and (C <= 1024 or (size == 4 and C > 4096))
+    few = C <= 16 or (size == 8 and wide)
+    E, vec = (32 if few else 64) // size, 16 // size if wide else 1
+    t = team(E, 256 if few else 512)
+    if t:
+        names.update("norm_backward_kernel<%s, %d, %d, %d, %s, false>" % (kind, vec, E // vec, t, one) for one in ("false", "true"))
+    elif C <= 256 * (64 // size) * 8:
+        large, small = -(-C // (512 * (64 // size))), -(-C // (256 * (64 // size)))
+        names.add("norm_backward_kernel<%s, 1, %d, %d, false, true>" % (kind, 64 // size, 512 if small == 2 * large else 256))
+    else:
+        names.update(("norm_backward_long_kernel<%s>" % kind, "norm_columns_kernel<%s>" % kind))
+    names.add("norm_fold_kernel<%s, %d>" % (kind, 16 // size if 2 * C * size % 16 == 0 else 1))
+    return names
+
+
+@pytest.mark.skipif(shutil.which("nm") is None, reason="needs nm")
+def test_every_layer_norm_kernel_can_be_launched():
+    """The library holds the kernels that some rows lead to, and no others."""
+    built = subprocess.run(["nm", "-C", build.LIB], capture_output=True, text=True, check=True).stdout
+    built = set(re.findall(r"\bnorm_\w+_kernel<[\w, ]+>", built))
+    reached = set()
+    for C in list(range(1, 2100)) + [2 ** k + d for k in range(11, 17) for d in (-1, 0, 1, 4)] + [12288, 12289, 24576, 24577, 24580]:
+        for kind in ("float", "double"):
+            for aligned in (False, True):
+                reached |= _norm_kernels(C, kind, aligned)
+    assert built == reached
