@@ -695,3 +695,92 @@ def test_what_is_said_of_a_wait_in_vain(rt, R, C):
     text = runtime.last_error()
     assert failed and "code 9" in text and "8-bit product" in text and "copy of a row or another block's sums" in text
     runtime.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------
+# sums that are exact, so that a term that is lost or counted twice cannot hide behind the roundings of the others
+# ------------------------------------------------------------------------------------------------
+EXACT_COLS = [2, 3, 5, 8, 17, 33, 65, 100, 300, 1001, 1028, 2047, 4096, 4097, 8192, 8193, 8196, 9001, 12289, 16384, 16385, 20001, 24577, 28676, 32768, 32769]
+
+
+def _columns(C, rs):
+    """All columns of a short row; of a long one those where the parts of 2 to 8 blocks or a thread's share may begin or end, and others."""
+    if C <= 1100:
+        return np.arange(C)
+    parts = [k * (-(-C // b // 4) * 4 if exact else -(-C // b)) for b in range(2, 9) for k in range(1, b) for exact in (False, True)]
+    near = [p + d for p in parts + [0, C, 1024, 2048, 4096, 8192, 16384] for d in range(-4, 5)]
+    return np.unique([c for c in near if 0 <= c < C] + list(rs.randint(0, C, 150)))
+
+
+def _signs(R, C, zero):
+    """Rows of +1 and -1 whose sum is 0; with an odd number of columns column `zero` of the row is 0."""
+    x = np.tile(np.where(np.arange(C) % 2, -1.0, 1.0), (R, 1))
+    if C % 2:
+        for r in range(R):
+            rest = np.arange(C) != zero[r]
+            x[r, rest], x[r, zero[r]] = np.where(np.arange(C - 1) % 2, -1.0, 1.0), 0
+    return x
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("C", EXACT_COLS)
+def test_every_column_counts_once_in_the_statistics(rt, C, dtype):
+    """One element of 1024 in a row of zeros, at every place: the result is sqrt(C - 1) there and -1 / sqrt(C - 1) elsewhere. The
+    mean's sum is exact; the squares are positive terms, off by three roundings each and at most 64 additions one behind the
+    other (16 or 33 of a thread, 10 of a block, 8 of a cluster); the root halves what the variance is off by: 45 roundings."""
+    at = _columns(C, np.random.RandomState(C))
+    x = np.zeros((len(at), C), dtype)
+    x[np.arange(len(at)), at] = 1024
+    want = np.full(x.shape, -1 / np.sqrt(C - 1.0))
+    want[np.arange(len(at)), at] = np.sqrt(C - 1.0)
+    y = _forward(x, np.ones(C, dtype), np.zeros(C, dtype), 0.0)
+    assert (np.abs(y - want) <= 45 * ref.U[dtype] * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("C", EXACT_COLS)
+def test_every_column_counts_once_in_the_gradients_sums(rt, C, dtype):
+    """Rows of +1 and -1 and a gradient that is 1024 in one place, every one in its row: all sums have one term or are whole
+    numbers, so what is left are the roundings of the formula, below 40 of the mean's term and 16 of the element's own."""
+    at = _columns(C, np.random.RandomState(C))
+    R = len(at)
+    x, own = _signs(R, C, np.where(at < C // 2, C - 1, 0)), (np.arange(R), at)
+    gain = 2.0 ** (np.arange(C) % 3)
+    gy = np.zeros((R, C))
+    gy[own] = 1024
+    rstd = np.sqrt(C / (C - C % 2))
+    d = 1024 * gain[at][:, None]
+    want = -rstd * d / C * (1 + x * x[own][:, None] * rstd ** 2)
+    want[own] += rstd * d[:, 0]
+    bound = 40 * ref.U[dtype] * rstd * d / C + np.zeros((R, C))
+    bound[own] += 16 * ref.U[dtype] * rstd * d[:, 0]
+    dx = _backward(x.astype(dtype), gain.astype(dtype), gy.astype(dtype), 0.0)[0]
+    assert (np.abs(dx - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["f4", "f8"])
+@pytest.mark.parametrize("R,C", [(7, 100), (64, 256), (3000, 4), (5001, 17), (4099, 33), (2000, 64), (1025, 300), (1000, 1001), (130, 2048), (600, 4096), (201, 4097),
+                                 (200, 8192), (300, 8193), (333, 12289), (90, 24580), (3, 32769), (150, 33000)])
+def test_every_row_counts_once_in_the_columns_sums(rt, R, C, dtype):
+    """Every row's gradient has one term, a power of two, in one column, each column's terms are different powers: the bias's gradient
+    is exact, and the gain's is off by at most 20 roundings, where a row that is missing or counted twice is 1 / 4095 or more."""
+    x = _signs(R, C, np.full(R, C - 1))
+    xh = x[0] * np.sqrt(C / (C - C % 2))
+    for first in range(0, R, 12 * C):
+        rows = np.arange(first, min(R, first + 12 * C))
+        gy = np.zeros((R, C))
+        gy[rows, rows % C] = 2.0 ** ((rows - first) // C)
+        want = gy.sum(0)
+        _dx, dgain, dbias = _backward(x.astype(dtype), np.ones(C, dtype), gy.astype(dtype), 0.0)
+        assert np.array_equal(dbias, want)
+        assert (np.abs(dgain - want * xh) <= 20 * ref.U[dtype] * np.abs(want * xh)).all()
+
+
+@pytest.mark.parametrize("C", [2, 17, 65, 300, 1001, 8192, 8193, 16384, 16385, 20480, 20481, 30001])
+def test_every_column_counts_in_a_rows_scale(rt, C):
+    """Rows of ones with one -254, at every place: scale 2, codes of a half that is rounded to 0."""
+    at = _columns(C, np.random.RandomState(C))
+    own = (np.arange(len(at)), at)
+    x, codes = np.ones((len(at), C), "f4"), np.zeros((len(at), -(-C // 16) * 16), "i1")
+    x[own], codes[own] = -254, -127
+    _same(_quantize(x), (codes, np.full(len(at), 2, "f4")))
