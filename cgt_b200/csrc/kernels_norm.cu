@@ -4,6 +4,7 @@
 #include "tc_util.h"
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -828,10 +829,13 @@ int norm_backward(const T* x, const T* gain, const T* gy, long R, long C, double
   return 0;
 }
 
-int norm_extents(const char* who, long R, long C, double eps) {
+int norm_extents(const char* who, int dtype, long R, long C, double eps) {
   if (R < 0 || C < 0) return fail("%s: negative extent", who);
   if (C > 0x7fffffffL) return fail("%s: rows of %ld elements are too long (at most 2^31 - 1)", who, C);
   if (!(eps >= 0) || std::isinf(eps)) return fail("%s: epsilon has to be a finite number that is not negative", who);
+  // rounded to 0 or infinity it would turn rows of equal values into NaN or all rows into the bias
+  if (dtype == cgtb_f4 && eps != 0 && !(eps >= FLT_MIN && eps <= FLT_MAX)) return fail("%s: epsilon %g is not a normal float32 number", who, eps);
+  if (eps != 0 && eps < DBL_MIN) return fail("%s: epsilon %g is not a normal number", who, eps);
   return 0;
 }
 
@@ -1023,7 +1027,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_rows_long_kernel(const 
 
 CGTB_API int cgtb_layer_norm_forward(int dtype, const void* x, long R, long C, const void* gain, const void* bias, double epsilon, void* y) {
   if (!require_runtime("cgtb_layer_norm_forward")) return 1;
-  if (norm_extents("cgtb_layer_norm_forward", R, C, epsilon)) return 1;
+  if (norm_extents("cgtb_layer_norm_forward", dtype, R, C, epsilon)) return 1;
   if (R == 0 || C == 0) return 0;
   if (dtype == cgtb_f4) return norm_forward((const float*)x, R, C, (const float*)gain, (const float*)bias, epsilon, (float*)y);
   if (dtype == cgtb_f8) return norm_forward((const double*)x, R, C, (const double*)gain, (const double*)bias, epsilon, (double*)y);
@@ -1033,7 +1037,7 @@ CGTB_API int cgtb_layer_norm_forward(int dtype, const void* x, long R, long C, c
 CGTB_API int cgtb_layer_norm_backward(int dtype, const void* x, const void* gain, const void* gy, long R, long C, double epsilon, void* dx, void* dgain,
                                       void* dbias) {
   if (!require_runtime("cgtb_layer_norm_backward")) return 1;
-  if (norm_extents("cgtb_layer_norm_backward", R, C, epsilon)) return 1;
+  if (norm_extents("cgtb_layer_norm_backward", dtype, R, C, epsilon)) return 1;
   if (dtype != cgtb_f4 && dtype != cgtb_f8) return fail("cgtb_layer_norm_backward: unsupported dtype %d", dtype);
   if (C == 0) return 0;
   if (R == 0) {   // sums of no rows

@@ -1,6 +1,8 @@
 """Layer norm over an array's last axis, with its gradients. Not in the reference, whose only norm is cross_channel_lrn."""
 import ctypes
 
+import numpy as np
+
 from .. import core
 
 
@@ -30,6 +32,9 @@ class LayerNorm(core.Op):
 
     def typ_apply(self, input_types):
         _check("layer_norm", input_types[0], input_types[1:])
+        info = np.finfo(input_types[0].dtype)
+        if self.epsilon and not float(info.tiny) <= self.epsilon <= float(info.max):
+            raise ValueError("epsilon has to be 0 or a normal number of type %s, got %s" % (input_types[0].dtype, self.epsilon))
         return input_types[0]
 
     def pullback(self, inputs, output, gout):
@@ -67,6 +72,6 @@ class LayerNormBackward(core.Op):
 
 def layer_norm(x, gain, bias, epsilon=1e-5):
     """x with every row along its last axis brought to mean 0 and variance 1, then scaled and shifted by the vectors `gain`
-    and `bias`, which have one value per column. A row of equal values gives `bias` (epsilon 0 makes it NaN).
-    Gradients of gradients are refused."""
+    and `bias`, which have one value per column. A row of equal values gives `bias` (epsilon 0 makes it NaN); any other epsilon
+    is a normal number of x's type, in float32 1.2e-38 or more. Gradients of gradients are refused."""
     return core.Result(LayerNorm(epsilon), [x, gain, bias])

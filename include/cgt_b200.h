@@ -198,7 +198,8 @@ int cgtb_lrn_backward(int dtype, const void* x, const void* top, const void* sca
  * Backward, with xh = (x - m) / sqrt(v + epsilon) and d = gy * gain:
  *   dx = (d - mean(d) - xh * mean(d * xh)) / sqrt(v + epsilon), dgain[c] = sum_r gy * xh, dbias[c] = sum_r gy.
  * The backward pass takes x and not y or saved statistics: it reads x anyway and forms them again. float32 and float64,
- * sums in the arrays' type, always in the same order. Any R and C >= 0; results may not overlap operands. */
+ * sums in the arrays' type, always in the same order. epsilon: 0 or a normal number of that type. Any R and C >= 0; results may
+ * not overlap operands. */
 int cgtb_layer_norm_forward(int dtype, const void* x, long R, long C, const void* gain, const void* bias, double epsilon, void* y);
 int cgtb_layer_norm_backward(int dtype, const void* x, const void* gain, const void* gy, long R, long C, double epsilon, void* dx,
                              void* dgain, void* dbias);

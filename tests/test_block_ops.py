@@ -306,3 +306,18 @@ def test_every_layer_norm_kernel_can_be_launched():
             for aligned in (False, True):
                 reached |= _norm_kernels(C, kind, aligned)
     assert built == reached
+
+
+def test_epsilons_that_the_type_does_not_hold():
+    """They would be rounded to 0, which makes rows of equal values NaN, or to infinity."""
+    x, v = cgt.matrix("x"), cgt.vector("v")
+    for epsilon in (1e-60, 1e-39, 1e39):
+        with pytest.raises(ValueError, match="normal number of type f4"):
+            nn.layer_norm(x, v, v, epsilon=epsilon)
+    for epsilon in (0.0, 1.2e-38, 3e38):
+        nn.layer_norm(x, v, v, epsilon=epsilon)
+    with cgt.scoped_update_config(precision="double"):
+        x, v = cgt.matrix("x"), cgt.vector("v")
+        nn.layer_norm(x, v, v, epsilon=1e-60)
+        with pytest.raises(ValueError, match="normal number of type f8"):
+            nn.layer_norm(x, v, v, epsilon=1e-310)

@@ -784,3 +784,17 @@ def test_every_column_counts_in_a_rows_scale(rt, C):
     x, codes = np.ones((len(at), C), "f4"), np.zeros((len(at), -(-C // 16) * 16), "i1")
     x[own], codes[own] = -254, -127
     _same(_quantize(x), (codes, np.full(len(at), 2, "f4")))
+
+
+def test_epsilons_at_the_ends_of_the_type(rt):
+    """Rows of equal values are the bias down to the smallest epsilon that is taken; smaller ones are refused."""
+    L = runtime.lib()
+    for (dtype, small, large) in (("f4", 1.2e-38, 3e38), ("f8", 2.3e-308, 1e308)):
+        x, bias = np.full((3, 40), 5, dtype), np.arange(40).astype(dtype)
+        for eps in (small, large):
+            assert np.array_equal(_forward(x, np.ones(40, dtype), bias, eps), np.tile(bias, (3, 1)))
+        d = Dev(x)
+        for eps in (small / 10, 1e-320, large * 10):
+            assert L.cgtb_layer_norm_forward(code(dtype), d.ptr, 3, 40, d.ptr, d.ptr, eps, d.ptr) != 0 and "epsilon" in runtime.last_error()
+            assert L.cgtb_layer_norm_backward(code(dtype), d.ptr, d.ptr, d.ptr, 3, 40, eps, d.ptr, d.ptr, d.ptr) != 0
+        assert np.array_equal(d.get(), x)
