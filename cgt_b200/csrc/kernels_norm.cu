@@ -1061,7 +1061,8 @@ CGTB_API int cgtb_dropout(int dtype, const void* x, long n, double p, const int6
   if (n < 0) return fail("cgtb_dropout: negative extent");
   if (dtype != cgtb_f4 && dtype != cgtb_f8) return fail("cgtb_dropout: unsupported dtype %d", dtype);
   if (n == 0) return 0;
-  // a word below the threshold drops its element; the largest p below 1 rounds to 2^32, which no word reaches
+  // A word below the threshold drops its element. p above 1 - 2^-33 would round to 2^32, which is no 32-bit number: there the
+  // threshold stays at 2^32 - 1, and the element of the largest word is kept
   const double t = std::nearbyint(p * 4294967296.0);
   const uint32_t threshold = t >= 4294967295.0 ? 4294967295u : (uint32_t)t;
   const double scale = 1.0 / (1.0 - p);
@@ -1088,6 +1089,8 @@ CGTB_API int cgtb_quantize_rows(const float* x, long R, long C, int8_t* codes, f
     if (wide) launch(std::true_type(), elements, team);
     else launch(std::false_type(), elements, team);
   };
+  // Up to 16384 codes 16 elements a thread, up to 20480 20, which fill the 64 registers that 1024 threads leave each (32 bytes are
+  // spilled); longer rows are read twice: 2000 x 16384 29 us, x 20480 35 us, x 20496 84 us.
   bool held = with_team<16, 1, 1024>(Cp, [&](auto team) { either(std::integral_constant<int, 16>(), team); });
   if (!held && Cp <= 1024 * 20) {
     either(std::integral_constant<int, 20>(), std::integral_constant<int, 1024>());

@@ -211,7 +211,7 @@ int cgtb_layer_norm_selftest_waits(long cycles);
 
 /* Dropout of n values, float32 or float64: y[i] = x[i] / (1 - p), or 0 where the element is dropped, whatever x[i] is. No mask
  * is stored: element i is dropped where word i % 4 of the Philox4x32-10 block with key (seed, seed >> 32) and counter
- * (i / 4, i / 4 >> 32, step, site) is below round(p * 2^32). state: two int64 in device memory, seed and step, read by the
+ * (i / 4, i / 4 >> 32, step, site) is below min(round(p * 2^32), 2^32 - 1). state: two int64 in device memory, seed and step, read by the
  * kernel, so that a captured graph drops other elements when its step has changed; the masks repeat after 2^32 steps. The
  * gradient is the same call on the gradient of y. 0 <= p < 1; y may be x. */
 int cgtb_dropout(int dtype, const void* x, long n, double p, const int64_t* state, unsigned site, void* y);
