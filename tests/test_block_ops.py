@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 
 import cgt_b200 as cgt
-from cgt_b200 import build, compilation, core, nn
+from cgt_b200 import build
+from cgt_b200 import compilation, core, nn
 from cgt_b200.nn_ops import dropout as dropout_ops
 from cgt_b200.nn_ops import int8 as int8_ops
 from cgt_b200.nn_ops import layer_norm as norm_ops
